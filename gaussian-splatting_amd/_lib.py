@@ -21,6 +21,31 @@ class GsAdamGroup(C.Structure):
                 ("grad_row_stride", _ll), ("row_len", _i), ("reserved", _i), ("lr", _d)]
 
 
+class GsAdamWTensor(C.Structure):
+    """struct GsAdamWTensor of include/gsplat.h"""
+    _fields_ = [("param", _vp), ("grad", _vp), ("param_low", _vp), ("exp_avg", _vp), ("exp_avg_sq", _vp), ("step_dev", _vp),
+                ("lr_dev", _vp), ("rows", _ll), ("grad_row_stride", _ll), ("step", _ll), ("lr", _d), ("beta1", _d),
+                ("beta2", _d), ("eps", _d), ("weight_decay", _d), ("row_len", _i), ("seed", C.c_uint32),
+                ("index", C.c_uint32), ("reserved", _i)]
+
+
+class GsGradTensor(C.Structure):
+    """struct GsGradTensor of include/gsplat.h"""
+    _fields_ = [("grad", _vp), ("rows", _ll), ("row_stride", _ll), ("row_len", _i), ("bf16", _i)]
+
+
+class GsAdamWRows(C.Structure):
+    """struct GsAdamWRows of include/gsplat.h"""
+    _fields_ = [("src_exp_avg", _vp), ("src_exp_avg_sq", _vp), ("src_param_low", _vp), ("dst_exp_avg", _vp),
+                ("dst_exp_avg_sq", _vp), ("dst_param_low", _vp), ("row_len", _i), ("reserved", _i)]
+
+
+class GsAdamWUnpack(C.Structure):
+    """struct GsAdamWUnpack of include/gsplat.h"""
+    _fields_ = [("codes", _vp), ("scales", _vp), ("param_bf16", _vp), ("param_low", _vp), ("exp_avg", _vp),
+                ("exp_avg_sq", _vp), ("param", _vp), ("numel", _ll)]
+
+
 class GsPlyLayout(C.Structure):
     """struct GsPlyLayout of include/gsplat.h"""
     _fields_ = [("num_vertices", _ll), ("data_offset", _ll), ("stride_bytes", _i), ("sh_rest_count", _i),
@@ -74,6 +99,12 @@ PROTOTYPES = {
     "gs_nearest_dist2_workspace_bytes": (_sz, [_ll]),
     "gs_nearest_dist2": (_i, [_ll, _vp, _vp, _vp, _sz, _vp, _vp]),
     "gs_adam_densify_step": (_i, [_i, C.POINTER(GsAdamGroup), _d, _d, _d, _ll, _ll, _i] + [_vp] * 6),
+    "gs_adamw_block": (_i, []),
+    "gs_adamw_step": (_i, [_i, C.POINTER(GsAdamWTensor), _i, _i, _i, _vp, _d, _vp, _vp]),
+    "gs_grad_norm_workspace_bytes": (_sz, [_i, C.POINTER(GsGradTensor)]),
+    "gs_grad_norm": (_i, [_i, C.POINTER(GsGradTensor), _vp, _vp, _sz, _vp]),
+    "gs_adamw_gather_rows": (_i, [_i, C.POINTER(GsAdamWRows), _i, _ll, _ll, _vp, _vp]),
+    "gs_adamw_unpack": (_i, [_i, C.POINTER(GsAdamWUnpack), _vp]),
 }
 
 _lib = None

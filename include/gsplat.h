@@ -315,6 +315,95 @@ int gs_adam_densify_step(int num_groups, const GsAdamGroup* groups, double beta1
                          void* stream);
 
 /*
+ * AdamW over many tensors (fp32 or bf16 parameters, moments in 32 or in 8 bits), one launch per 32 tensors:
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m' / (sqrt(v') / sqrt(1 - beta2^t) + eps)
+ * with m' = beta1 m + (1 - beta1) g, v' = beta2 v + (1 - beta2) g^2, everything in fp32 (32-bit moments: operation by
+ * operation torch.optim.AdamW's).  `tensors` is a HOST array of device pointers; param, param_low and the moments are contiguous,
+ * grad (the parameter's type) is a (rows, row_len) matrix that may have a row stride in elements (0 = contiguous).
+ *   state_bits 32: exp_avg, exp_avg_sq fp32.
+ *   state_bits 8:  exp_avg points to the code pairs, uint8 (rows * row_len, 2): (code of m, code of sqrt(v)); exp_avg_sq to the
+ *                  scale pairs, fp32 (ceil(rows * row_len / GS_ADAMW_BLOCK), 2): (largest |m|, largest sqrt(v)) of
+ *                  64 consecutive elements.  m: bit 7 = sign, c = bits 0..6; c = 0 is 0, else
+ *                  scale * float_with_bits(0x3F800000 - (127 - c) * 2^20).  sqrt(v): c = 0 is 0, else
+ *                  scale * float_with_bits(0x3F800000 - (255 - c) * 2^19).  stochastic_rounding != 0: a value between two
+ *                  levels goes up with the probability of its place between them; the random bits are a hash of (seed,
+ *                  index, t, element).  0: nearest.  A block that takes in a NaN reads as NaN wherever it is not 0.
+ *   param_bf16:    the fp32 value is (bits(param) << 16) + param_low; both are updated.  NULL for fp32 parameters.
+ *   grad_norm:     device scalar or NULL; with it every gradient is multiplied by min(1, max_norm / (grad_norm + 1e-6)).
+ *   t:             `step` (host, the count after this update) or, for calls that are captured and replayed, *step_dev (device,
+ *                  the count before it; incremented) with `scalars` = 4 floats of device workspace per tensor, 16-byte
+ *                  aligned, on all tensors of a call or on none.  lr_dev (device, with step_dev only) replaces lr.
+ */
+#define GS_ADAMW_BLOCK 64
+typedef struct GsAdamWTensor {
+    void* param;
+    const void* grad;
+    int16_t* param_low;
+    void* exp_avg;
+    float* exp_avg_sq;
+    float* step_dev;
+    const float* lr_dev;
+    long long rows;
+    long long grad_row_stride;
+    long long step;
+    double lr, beta1, beta2, eps, weight_decay;
+    int row_len;
+    uint32_t seed, index;
+    int reserved;
+} GsAdamWTensor;
+int gs_adamw_block(void);        /* GS_ADAMW_BLOCK */
+int gs_adamw_step(int num_tensors, const GsAdamWTensor* tensors, int param_bf16, int state_bits, int stochastic_rounding,
+                  const float* grad_norm, double max_norm, float* scalars, void* stream);
+
+/*
+ * norm = sqrt of the sum of squares over all tensors (fp32 or bf16 (rows, row_len) matrices, row_stride in elements,
+ * 0 = contiguous): accumulated in fp64 in an order that depends on the sizes alone, rounded once.  norm: one device float.
+ */
+typedef struct GsGradTensor {
+    const void* grad;
+    long long rows;
+    long long row_stride;
+    int row_len;
+    int bf16;
+} GsGradTensor;
+size_t gs_grad_norm_workspace_bytes(int num_tensors, const GsGradTensor* tensors);
+int gs_grad_norm(int num_tensors, const GsGradTensor* tensors, float* norm, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Rows of AdamW states: row i of every dst is row index[i] of its src (src_rows rows of row_len elements); an index outside
+ * 0..src_rows-1 gives a fresh row (zeros).  8-bit states get the scales of their new blocks and are rounded to
+ * the nearest level.  src and dst must not overlap.  param_low: NULL where there is none.
+ */
+typedef struct GsAdamWRows {
+    const void* src_exp_avg;
+    const float* src_exp_avg_sq;
+    const int16_t* src_param_low;
+    void* dst_exp_avg;
+    float* dst_exp_avg_sq;
+    int16_t* dst_param_low;
+    int row_len;
+    int reserved;
+} GsAdamWRows;
+int gs_adamw_gather_rows(int num_tensors, const GsAdamWRows* tensors, int state_bits, long long src_rows, long long dst_rows,
+                         const int64_t* index, void* stream);
+
+/*
+ * The fp32 values behind packed states: codes + scales -> exp_avg, exp_avg_sq (= the square of the second level) when codes is
+ * not NULL; (param_bf16, param_low) -> param when param_bf16 is not NULL.
+ */
+typedef struct GsAdamWUnpack {
+    const uint8_t* codes;
+    const float* scales;
+    const void* param_bf16;
+    const int16_t* param_low;
+    float* exp_avg;
+    float* exp_avg_sq;
+    float* param;
+    long long numel;
+} GsAdamWUnpack;
+int gs_adamw_unpack(int num_tensors, const GsAdamWUnpack* tensors, void* stream);
+
+/*
  * Trained-model PLY <-> device layout.  Replaces GaussianModel.load_ply / save_ply
  * (scene/gaussian_model.py:377-459, :333-375; attribute order :316-331; plyfile underneath).
  * gs_ply_parse_header (host): reads the ASCII header of a binary_little_endian PLY from the first n_bytes of
