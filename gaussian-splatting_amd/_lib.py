@@ -100,11 +100,12 @@ PROTOTYPES = {
     "gs_nearest_dist2": (_i, [_ll, _vp, _vp, _vp, _sz, _vp, _vp]),
     "gs_adam_densify_step": (_i, [_i, C.POINTER(GsAdamGroup), _d, _d, _d, _ll, _ll, _i] + [_vp] * 6),
     "gs_adamw_block": (_i, []),
-    "gs_adamw_step": (_i, [_i, C.POINTER(GsAdamWTensor), _i, _i, _i, _vp, _d, _vp, _vp]),
-    "gs_grad_norm_workspace_bytes": (_sz, [_i, C.POINTER(GsGradTensor)]),
-    "gs_grad_norm": (_i, [_i, C.POINTER(GsGradTensor), _vp, _vp, _sz, _vp]),
-    "gs_adamw_gather_rows": (_i, [_i, C.POINTER(GsAdamWRows), _i, _ll, _ll, _vp, _vp]),
-    "gs_adamw_unpack": (_i, [_i, C.POINTER(GsAdamWUnpack), _vp]),
+    # tables of descriptors go in as packed bytes or as ctypes arrays of the structs above
+    "gs_adamw_step": (_i, [_i, _vp, _i, _i, _i, _vp, _d, _vp, _vp]),
+    "gs_grad_norm_workspace_bytes": (_sz, [_i, _vp]),
+    "gs_grad_norm": (_i, [_i, _vp, _vp, _vp, _sz, _vp]),
+    "gs_adamw_gather_rows": (_i, [_i, _vp, _i, _ll, _ll, _vp, _vp]),
+    "gs_adamw_unpack": (_i, [_i, _vp, _vp]),
 }
 
 _lib = None

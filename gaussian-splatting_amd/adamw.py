@@ -16,7 +16,6 @@
 """
 from __future__ import annotations
 
-import ctypes as C
 import struct
 
 import torch
@@ -26,17 +25,33 @@ from .optimizer import FusedAdam
 from .profiling import stage as _stage
 
 BLOCK = 64                                       # GS_ADAMW_BLOCK: elements that share a pair of scales
-_STEP = struct.Struct("@7P3q5diIIi")             # GsAdamWTensor
-_GRAD = struct.Struct("@P2q2i")                  # GsGradTensor
-_TYPES = (torch.float32, torch.bfloat16)
+_F32, _BF16 = torch.float32, torch.bfloat16
+
+# The descriptors of include/gsplat.h as packed bytes: a step describes every tensor anew, and a small model's step takes as long as that does.
+_STEP = struct.Struct("@7P3q5diIIi").pack        # GsAdamWTensor
+_GRAD = struct.Struct("@P2q2i").pack             # GsGradTensor
+_ROWS = struct.Struct("@6P2i").pack              # GsAdamWRows
+_UNPACK = struct.Struct("@7Pq").pack             # GsAdamWUnpack
 
 
-def _ptr(t):
-    return None if t is None else C.c_void_p(t.data_ptr())
+class _On:
+    """The device context of a call, entered only where the device is not the current one already."""
+    __slots__ = ("ctx",)
+
+    def __init__(self, dev):
+        self.ctx = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.ctx is not None:
+            self.ctx.__enter__()
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
 
 
-def _table(struct_type, packed):
-    return (struct_type * len(packed)).from_buffer(bytearray(b"".join(packed)))
+def _stream():
+    return torch.cuda.current_stream().cuda_stream
 
 
 def _matrix(g):
@@ -52,29 +67,27 @@ def _matrix(g):
         else:
             if row_len <= g.stride(0) and 0 < row_len < 1 << 31:
                 return g, g.shape[0], row_len, g.stride(0)
-    return g.contiguous(), g.numel(), 1, 0
+    return g.detach().contiguous(), g.numel(), 1, 0
 
 
 def _check_grad(g, what):
-    if g.layout != torch.strided or not g.is_cuda:
+    if g.layout is not torch.strided or not g.is_cuda:
         raise RuntimeError(f"{what} must be a dense tensor on the GPU (no CPU path)")
-    if g.dtype not in _TYPES:
+    if g.dtype is not _F32 and g.dtype is not _BF16:
         raise RuntimeError(f"{what} must be float32 or bfloat16, not {g.dtype}")
 
 
-def _norm(mats, dev):
-    """Launches gs_grad_norm over (matrix, is_bf16) pairs on the current stream of `dev`, the current device."""
+def _norm(mats, dev, stream):
+    """Launches gs_grad_norm over matrices of _matrix() on `stream` of `dev`, the current device."""
     lib = _lib.load()
-    arr = _table(_lib.GsGradTensor, [_GRAD.pack(g.data_ptr(), rows, stride, row_len, bf16) for (g, rows, row_len, stride), bf16 in mats])
-    size = lib.gs_grad_norm_workspace_bytes(len(mats), arr)
+    table = b"".join([_GRAD(g.data_ptr(), rows, stride, row_len, g.dtype is _BF16) for g, rows, row_len, stride in mats])
+    size = lib.gs_grad_norm_workspace_bytes(len(mats), table)
     ws = torch.empty(max(size, 8), dtype=torch.uint8, device=dev)
-    out = torch.empty((), dtype=torch.float32, device=dev)
-    _lib.check(lib.gs_grad_norm(len(mats), arr, _ptr(out), _ptr(ws), size, C.c_void_p(torch.cuda.current_stream().cuda_stream)),
-               "gs_grad_norm")
+    out = torch.empty((), dtype=_F32, device=dev)
+    _lib.check(lib.gs_grad_norm(len(mats), table, out.data_ptr(), ws.data_ptr(), size, stream), "gs_grad_norm")
     return out
 
 
-@torch.no_grad()
 def grad_norm(grads):
     """sqrt of the sum of squares over all given tensors (None is skipped) as a 0-d float32 GPU tensor.
 
@@ -84,12 +97,13 @@ def grad_norm(grads):
     grads = [grads] if torch.is_tensor(grads) else [g for g in grads if g is not None]
     if not grads:
         raise ValueError("grad_norm needs at least one tensor")
+    dev = grads[0].device
     for g in grads:
         _check_grad(g, "grad_norm: a gradient")
-        if g.device != grads[0].device:
+        if g.device != dev:
             raise RuntimeError("grad_norm: all gradients must live on one device")
-    with torch.cuda.device(grads[0].device), _stage("grad_norm"):
-        return _norm([(_matrix(g), g.dtype == torch.bfloat16) for g in grads], grads[0].device)
+    with _On(dev), _stage("grad_norm"):
+        return _norm([_matrix(g) for g in grads], dev, _stream())
 
 
 class FusedAdamW(torch.optim.AdamW):
@@ -126,7 +140,6 @@ class FusedAdamW(torch.optim.AdamW):
             self._complete(self.param_groups[-1])
 
     # ---- the step ---------------------------------------------------------------------------------------------------
-    @torch.no_grad()
     def step(self, closure=None, *, max_norm=None, grad_norm=None):
         """One AdamW update of every parameter that has a .grad (others are skipped, as in torch).
 
@@ -146,71 +159,76 @@ class FusedAdamW(torch.optim.AdamW):
         self.last_grad_norm = None
         if not work:
             return loss
-        if grad_norm is not None and (not torch.is_tensor(grad_norm) or grad_norm.device != dev or grad_norm.dtype != torch.float32
+        if grad_norm is not None and (not torch.is_tensor(grad_norm) or grad_norm.device != dev or grad_norm.dtype is not _F32
                                       or grad_norm.numel() != 1):
             raise ValueError("grad_norm must be one float32 on the parameters' device")
-        with torch.cuda.device(dev), _stage("adamw"):
-            capturing = torch.cuda.is_current_stream_capturing()
-            if capturing:
+        with _On(dev), _stage("adamw"):
+            if torch.cuda.is_current_stream_capturing():
                 self._check_capture(work)
-            mats = [_matrix(g) for _, _, _, g, _ in work]
+            stream = _stream()
+            mats = [_matrix(w[3]) for w in work]
             if max_norm is not None and grad_norm is None:
-                grad_norm = _norm([(m, g.dtype == torch.bfloat16) for m, (_, _, _, g, _) in zip(mats, work)], dev)
-            self._launch(work, mats, grad_norm, max_norm, dev)
+                grad_norm = _norm(mats, dev, stream)
+            self._launch(work, mats, grad_norm, max_norm, dev, stream)
         self.last_grad_norm = grad_norm
-        torch.autograd.graph.increment_version([p for _, p, _, _, _ in work])
+        torch.autograd.graph.increment_version([w[1] for w in work])
         return loss
 
     def _collect(self):
         """Everything that the step updates, checked before anything changes: [(group, param, index, grad, state or None)]."""
-        work, dev, index, spans = [], None, -1, []
+        work, dev, index, spans, states = [], None, -1, [], self.state
         for group in self.param_groups:
             if group["amsgrad"] or group["maximize"] or group["differentiable"]:
                 raise NotImplementedError("FusedAdamW: amsgrad / maximize / differentiable are not implemented")
             beta1, beta2 = group["betas"]
-            if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0 and group["eps"] >= 0.0 and group["state_bits"] in (8, 32)):
-                raise ValueError(f"FusedAdamW: betas {group['betas']}, eps {group['eps']}, state_bits {group['state_bits']}: betas are in "
+            bits = group["state_bits"]
+            if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0 and group["eps"] >= 0.0 and bits in (8, 32)):
+                raise ValueError(f"FusedAdamW: betas {group['betas']}, eps {group['eps']}, state_bits {bits}: betas are in "
                                  "[0, 1), eps is not negative, state_bits is 8 or 32")
             for p in group["params"]:
                 index += 1
                 g = p.grad
                 if g is None:
                     continue
-                if not p.is_cuda or p.dtype not in _TYPES or not p.is_contiguous():
+                dtype = p.dtype
+                if not p.is_cuda or dtype is not _F32 and dtype is not _BF16 or not p.is_contiguous():
                     raise RuntimeError("FusedAdamW needs contiguous float32 or bfloat16 parameters on the GPU (no CPU path)")
                 _check_grad(g, "FusedAdamW: a gradient")
-                if g.dtype != p.dtype or g.device != p.device:
-                    raise RuntimeError("FusedAdamW needs gradients of the parameter's type on its device")
                 if dev is None:
                     dev = p.device
-                elif dev != p.device:
-                    raise RuntimeError("FusedAdamW: all parameters must live on one device")
-                state = self.state.get(p) or None
+                if g.dtype is not dtype or p.device != dev or g.device != dev:
+                    raise RuntimeError("FusedAdamW: all parameters must live on one device, with gradients of their type there")
+                state = states.get(p) or None
                 if state is not None:
-                    self._check_state(p, state, group["state_bits"])
-                if p.numel():
-                    spans.append((p.data_ptr(), p.numel() * p.element_size()))
+                    self._check_state(p, state, bits)
+                n = p.numel()
+                if n:
+                    start = p.data_ptr()
+                    spans.append((start, start + n * (4 if dtype is _F32 else 2)))
                 work.append((group, p, index, g, state))
         spans.sort()
-        for (a, size), (b, _) in zip(spans, spans[1:]):
-            if a + size > b:
+        end = 0
+        for start, stop in spans:
+            if start < end:
                 raise RuntimeError("FusedAdamW: two parameters share memory (or one is listed twice)")
+            end = stop
         return work, dev
 
     @staticmethod
     def _check_state(p, state, bits):
+        dev, shape = p.device, p.shape
         if bits == 8:
             a, b = state.get("moment_codes"), state.get("moment_scales")
-            good = (a is not None and b is not None and a.dtype == torch.uint8 and a.shape == p.shape + (2,)
+            good = (a is not None and b is not None and a.dtype is torch.uint8 and a.shape == shape + (2,)
                     and b.shape == ((p.numel() + BLOCK - 1) // BLOCK, 2))
         else:
             a, b = state.get("exp_avg"), state.get("exp_avg_sq")
-            good = a is not None and b is not None and a.dtype == torch.float32 and a.shape == p.shape and b.shape == p.shape
-        low = state.get("param_low") if p.dtype == torch.bfloat16 else None
-        if p.dtype == torch.bfloat16:
-            good = good and low is not None and low.dtype == torch.int16 and low.shape == p.shape and low.is_contiguous() and low.device == p.device
-        if not good or b.dtype != torch.float32 or not (a.is_contiguous() and b.is_contiguous()) or a.device != p.device or b.device != p.device:
-            raise RuntimeError(f"FusedAdamW: optimizer state does not match its parameter (shape {tuple(p.shape)}, {p.dtype}, state_bits {bits}); "
+            good = a is not None and b is not None and a.dtype is _F32 and a.shape == shape and b.shape == shape
+        if p.dtype is _BF16:
+            low = state.get("param_low")
+            good = good and low is not None and low.dtype is torch.int16 and low.shape == shape and low.is_contiguous() and low.device == dev
+        if not good or b.dtype is not _F32 or not (a.is_contiguous() and b.is_contiguous()) or a.device != dev or b.device != dev:
+            raise RuntimeError(f"FusedAdamW: optimizer state does not match its parameter (shape {tuple(shape)}, {p.dtype}, state_bits {bits}); "
                                "replace_params() takes states along when rows are pruned or added")
 
     @staticmethod
@@ -234,42 +252,45 @@ class FusedAdamW(torch.optim.AdamW):
             if state is None or not (torch.is_tensor(state["step"]) and state["step"].is_cuda):
                 raise RuntimeError("FusedAdamW: run one step before the capture (states made during a capture would be cleared by every replay)")
 
-    def _launch(self, work, mats, norm, max_norm, dev):
+    def _launch(self, work, mats, norm, max_norm, dev, stream):
         lib = _lib.load()
         buckets, keep, counted = {}, [], []
         for (group, p, index, g, state), (gk, rows, row_len, stride) in zip(work, mats):
-            bits, on_gpu = group["state_bits"], bool(group["capturable"])
+            bits, on_gpu, bf16 = group["state_bits"], bool(group["capturable"]), p.dtype is _BF16
             if state is None:
                 state = self.state[p] = self._fresh_state(p, bits, on_gpu)
             lr, step, lr_dev, step_dev, t = group["lr"], state["step"], 0, 0, 0
             if on_gpu:
-                if not torch.is_tensor(step) or step.device != dev or step.dtype != torch.float32:
-                    step = state["step"] = torch.as_tensor(step, dtype=torch.float32).to(dev)
+                if not torch.is_tensor(step) or step.device != dev or step.dtype is not _F32:
+                    step = state["step"] = torch.as_tensor(step, dtype=_F32).to(dev)
                 step_dev = step.data_ptr()
                 if torch.is_tensor(lr) and lr.is_cuda:
-                    lr = lr.to(device=dev, dtype=torch.float32)
+                    lr = lr.detach().to(device=dev, dtype=_F32)
                     if lr.numel() != 1:
                         raise ValueError("FusedAdamW: lr must be one number")
                     keep.append(lr)
                     lr_dev, lr = lr.data_ptr(), 0.0
             else:
                 t = int(step) + 1
-                counted.append(state)
-            low = 0
-            if p.dtype == torch.bfloat16:
-                low = state["param_low"].data_ptr()
+                counted.append((state, step, t))
             a, b = (state["moment_codes"], state["moment_scales"]) if bits == 8 else (state["exp_avg"], state["exp_avg_sq"])
             beta1, beta2 = group["betas"]
-            buckets.setdefault((p.dtype == torch.bfloat16, bits, group["stochastic_rounding"], on_gpu), []).append(
-                _STEP.pack(p.data_ptr(), gk.data_ptr(), low, a.data_ptr(), b.data_ptr(), step_dev, lr_dev, rows, stride, t, float(lr),
-                           beta1, beta2, group["eps"], group["weight_decay"], row_len, group["seed"] & 0xFFFFFFFF, index, 0))
-        stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+            key = (bf16, bits, group["stochastic_rounding"], on_gpu)
+            if key not in buckets:
+                buckets[key] = []
+            buckets[key].append(_STEP(p.data_ptr(), gk.data_ptr(), state["param_low"].data_ptr() if bf16 else 0, a.data_ptr(), b.data_ptr(),
+                                      step_dev, lr_dev, rows, stride, t, float(lr), beta1, beta2, group["eps"], group["weight_decay"],
+                                      row_len, group["seed"] & 0xFFFFFFFF, index, 0))
         for (bf16, bits, stochastic, on_gpu), packed in buckets.items():
-            scalars = torch.empty(4 * len(packed), dtype=torch.float32, device=dev) if on_gpu else None
-            _lib.check(lib.gs_adamw_step(len(packed), _table(_lib.GsAdamWTensor, packed), bf16, bits, stochastic, _ptr(norm),
-                                         0.0 if max_norm is None else float(max_norm), _ptr(scalars), stream), "gs_adamw_step")
-        for state in counted:                    # after the launch: a refused call leaves the counts as they were
-            state["step"] += 1
+            scalars = torch.empty(4 * len(packed), dtype=_F32, device=dev) if on_gpu else None
+            _lib.check(lib.gs_adamw_step(len(packed), b"".join(packed), bf16, bits, stochastic, None if norm is None else norm.data_ptr(),
+                                         0.0 if max_norm is None else float(max_norm), None if scalars is None else scalars.data_ptr(),
+                                         stream), "gs_adamw_step")
+        for state, step, t in counted:           # after the launch: a refused call leaves the counts as they were
+            if torch.is_tensor(step):
+                step.fill_(t)
+            else:
+                state["step"] = t
 
     @torch.no_grad()
     def update_densify_stats(self, viewspace_grad=None, radii=None, xyz_gradient_accum=None, denom=None, max_radii2D=None):
@@ -287,7 +308,6 @@ class FusedAdamW(torch.optim.AdamW):
                     return group
         raise ValueError("not a parameter of this optimizer")
 
-    @torch.no_grad()
     def gather_state(self, params, index):
         """States for tensors whose row i is row ``index[i]`` of each of ``params``: a list of state dicts in their order.
 
@@ -299,14 +319,18 @@ class FusedAdamW(torch.optim.AdamW):
             return []
         if not torch.is_tensor(index) or index.dtype != torch.int64 or index.dim() != 1:
             raise ValueError("index must be a 1-d int64 tensor (of a mask: mask.nonzero()[:, 0])")
-        n, m = (params[0].shape[0] if params[0].dim() else -1), index.shape[0]
-        buckets, out, keep = {}, [], []
+        dev, m = params[0].device, index.shape[0]
+        n = params[0].shape[0] if params[0].dim() else -1
+        group_of = {q: group for group in self.param_groups for q in group["params"]}
+        buckets, out = {}, []
         for p in params:
             if p.dim() < 1 or p.shape[0] != n:
                 raise ValueError("gather_state: all params need the same number of rows")
-            if not p.is_cuda or p.device != params[0].device or index.device != p.device:
+            if not p.is_cuda or p.device != dev or index.device != dev:
                 raise RuntimeError("gather_state: params and index must live on one GPU (no CPU path)")
-            bits = self._group_of(p)["state_bits"]
+            if p not in group_of:
+                raise ValueError("not a parameter of this optimizer")
+            bits = group_of[p]["state_bits"]
             state = self.state.get(p) or None
             if state is None:
                 out.append({})
@@ -314,35 +338,30 @@ class FusedAdamW(torch.optim.AdamW):
             self._check_state(p, state, bits)
             step = state["step"]
             new = {"step": step.clone() if torch.is_tensor(step) else step}
-            shape = (m,) + tuple(p.shape[1:])
-            row_len = 1
-            for d in p.shape[1:]:
-                row_len *= d
+            row = p.shape[1:]
+            shape, row_len = (m,) + row, row.numel()
             if row_len >= 1 << 31:
                 raise ValueError(f"gather_state: rows of {row_len} elements are too long")
             if bits == 8:
-                names = ("moment_codes", "moment_scales")
-                new["moment_codes"] = torch.empty(shape + (2,), dtype=torch.uint8, device=p.device)
-                new["moment_scales"] = torch.empty(((m * row_len + BLOCK - 1) // BLOCK, 2), dtype=torch.float32, device=p.device)
+                a, b = state["moment_codes"], state["moment_scales"]
+                x = new["moment_codes"] = a.new_empty(shape + (2,))
+                y = new["moment_scales"] = b.new_empty(((m * row_len + BLOCK - 1) // BLOCK, 2))
             else:
-                names = ("exp_avg", "exp_avg_sq")
-                new["exp_avg"] = torch.empty(shape, dtype=torch.float32, device=p.device)
-                new["exp_avg_sq"] = torch.empty(shape, dtype=torch.float32, device=p.device)
-            low = state.get("param_low")
-            if low is not None:
-                new["param_low"] = torch.empty(shape, dtype=torch.int16, device=p.device)
+                a, b = state["exp_avg"], state["exp_avg_sq"]
+                x = new["exp_avg"] = a.new_empty(shape)
+                y = new["exp_avg_sq"] = a.new_empty(shape)
+            low_from = low_to = 0
+            if p.dtype is _BF16:
+                low_from, new["param_low"] = state["param_low"].data_ptr(), state["param_low"].new_empty(shape)
+                low_to = new["param_low"].data_ptr()
             if row_len:
-                buckets.setdefault(bits, []).append(_lib.GsAdamWRows(
-                    state[names[0]].data_ptr(), state[names[1]].data_ptr(), None if low is None else low.data_ptr(), new[names[0]].data_ptr(),
-                    new[names[1]].data_ptr(), None if low is None else new["param_low"].data_ptr(), row_len, 0))
+                buckets.setdefault(bits, []).append(_ROWS(a.data_ptr(), b.data_ptr(), low_from, x.data_ptr(), y.data_ptr(), low_to, row_len, 0))
             out.append(new)
         lib = _lib.load()
-        with torch.cuda.device(params[0].device), _stage("adamw_rows"):
+        with _On(dev), _stage("adamw_rows"):
             index = index.contiguous()
-            stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
             for bits, rows in buckets.items():
-                _lib.check(lib.gs_adamw_gather_rows(len(rows), (_lib.GsAdamWRows * len(rows))(*rows), bits, n, m, _ptr(index), stream),
-                           "gs_adamw_gather_rows")
+                _lib.check(lib.gs_adamw_gather_rows(len(rows), b"".join(rows), bits, n, m, index.data_ptr(), _stream()), "gs_adamw_gather_rows")
         return out
 
     def replace_params(self, old, new, index):
@@ -370,7 +389,6 @@ class FusedAdamW(torch.optim.AdamW):
                 self.state[q] = state
 
     # ---- what states stand for ----------------------------------------------------------------------------------------
-    @torch.no_grad()
     def unpacked(self, params=None, *, states=None):
         """[{"param", "exp_avg", "exp_avg_sq"}] in float32 for ``params`` (all that have a state), or for ``states`` as gather_state
         returns them (without "param").  What is kept in float32 already is returned itself, the rest is
@@ -384,38 +402,44 @@ class FusedAdamW(torch.optim.AdamW):
                 params = [p for group in self.param_groups for p in group["params"] if self.state.get(p)]
             pairs = [(p, self.state.get(p) or {}) for p in params]
         out, packed, dev = [], [], None
+        group_of = {q: group for group in self.param_groups for q in group["params"]} if states is None else None
         for p, s in pairs:
-            got, codes, low = {}, s.get("moment_codes"), s.get("param_low")
+            codes, got, numel = s.get("moment_codes"), {}, 0
+            entry = [0, 0, 0, 0, 0, 0, 0]
             if p is not None and s:
-                self._check_state(p, s, self._group_of(p)["state_bits"])
-            entry = _lib.GsAdamWUnpack()
+                if p not in group_of:
+                    raise ValueError("not a parameter of this optimizer")
+                self._check_state(p, s, group_of[p]["state_bits"])
             if codes is not None:
-                scales = s["moment_scales"]
-                if not (codes.is_cuda and codes.is_contiguous() and scales.is_contiguous()) or codes.dtype != torch.uint8 or \
-                        scales.dtype != torch.float32 or scales.shape != ((codes.numel() // 2 + BLOCK - 1) // BLOCK, 2) or scales.device != codes.device:
+                scales, here, numel = s["moment_scales"], codes.device, codes.numel() // 2
+                if p is None and (not (codes.is_cuda and codes.is_contiguous() and scales.is_contiguous()) or codes.dtype is not torch.uint8 or
+                                  scales.dtype is not _F32 or scales.device != here or codes.shape[-1:] != (2,) or
+                                  scales.shape != ((numel + BLOCK - 1) // BLOCK, 2)):
                     raise RuntimeError("unpacked: not a state of FusedAdamW on the GPU")
-                got["exp_avg"] = torch.empty(codes.shape[:-1], dtype=torch.float32, device=codes.device)
-                got["exp_avg_sq"] = torch.empty_like(got["exp_avg"])
-                entry.codes, entry.scales = codes.data_ptr(), scales.data_ptr()
-                entry.exp_avg, entry.exp_avg_sq, entry.numel = got["exp_avg"].data_ptr(), got["exp_avg_sq"].data_ptr(), got["exp_avg"].numel()
+                m = got["exp_avg"] = scales.new_empty(codes.shape[:-1])
+                v = got["exp_avg_sq"] = torch.empty_like(m)
+                entry[0], entry[1], entry[4], entry[5] = codes.data_ptr(), scales.data_ptr(), m.data_ptr(), v.data_ptr()
             elif s:
                 got["exp_avg"], got["exp_avg_sq"] = s["exp_avg"], s["exp_avg_sq"]
             if p is not None:
                 got["param"] = p.detach()
-                if p.dtype == torch.bfloat16 and low is not None:
-                    got["param"] = torch.empty(p.shape, dtype=torch.float32, device=p.device)
-                    entry.param_bf16, entry.param_low, entry.param, entry.numel = p.data_ptr(), low.data_ptr(), got["param"].data_ptr(), p.numel()
+                if p.dtype is _BF16:
+                    if s:
+                        here, numel, low = p.device, p.numel(), s["param_low"]
+                        x = got["param"] = torch.empty(p.shape, dtype=_F32, device=here)
+                        entry[2], entry[3], entry[6] = p.data_ptr(), low.data_ptr(), x.data_ptr()
+                    else:
+                        got["param"] = p.detach().float()
             out.append(got)
-            if entry.numel:
-                here = codes.device if codes is not None else p.device
-                if dev not in (None, here):
+            if numel:
+                if dev is None:
+                    dev = here
+                elif dev != here:
                     raise RuntimeError("unpacked: all tensors must live on one device")
-                dev = here
-                packed.append(entry)
+                packed.append(_UNPACK(*entry, numel))
         if packed:
-            with torch.cuda.device(dev), _stage("adamw_unpack"):
-                _lib.check(_lib.load().gs_adamw_unpack(len(packed), (_lib.GsAdamWUnpack * len(packed))(*packed),
-                                                       C.c_void_p(torch.cuda.current_stream().cuda_stream)), "gs_adamw_unpack")
+            with _On(dev), _stage("adamw_unpack"):
+                _lib.check(_lib.load().gs_adamw_unpack(len(packed), b"".join(packed), _stream()), "gs_adamw_unpack")
         return out
 
     # ---- checkpoints --------------------------------------------------------------------------------------------------

@@ -38,6 +38,22 @@ constexpr int AW_THREADS = 256;
 constexpr int AW_MAX_TENSORS = 32;      // tensors per launch: the table travels in the kernel arguments (4 KB)
 constexpr int AW_CHUNK = 2048;          // elements per workgroup, a multiple of AW_THREADS and of GS_ADAMW_BLOCK
 
+// A (rows, row_len) matrix as a chunk of consecutive elements sees it: where the chunk starts (the same for the whole workgroup, so
+// scalar arithmetic), and the row of an element `off` further on by one 32-bit multiply-high.  Chunks have at most 8192 elements.
+struct AwDivisor { unsigned long long magic; uint32_t len, magic32; };    // floor(2^64 / len) + 1, floor(2^32 / len) + 1; len 0: contiguous
+struct AwRows { long long row; uint32_t col, len, magic32; };
+struct AwPlace { uint32_t q, col; };                                      // rows after the chunk's first, column
+__device__ __forceinline__ AwRows aw_rows(long long base, const AwDivisor& d) {
+    const long long row = d.len == 1 ? base : (long long)__umul64hi((unsigned long long)base, d.magic);
+    return AwRows{row, (uint32_t)(base - row * d.len), d.len, d.magic32};
+}
+__device__ __forceinline__ AwPlace aw_place(const AwRows& r, uint32_t off) {
+    const uint32_t x = r.col + off;       // < len + 8192
+    if (r.len >= 8192u) return x >= r.len ? AwPlace{1u, x - r.len} : AwPlace{0u, x};
+    const uint32_t q = r.len == 1 ? x : __umulhi(x, r.magic32);          // exact: x * len < 2^28
+    return AwPlace{q, x - __umul24(q, r.len)};
+}
+
 struct AwTensor {
     void* p;
     const void* g;
@@ -46,8 +62,7 @@ struct AwTensor {
     float* v;                 // fp32 moments, or the scale pairs
     long long n;
     long long g_row_stride;
-    unsigned long long magic; // floor(2^64 / row_len) + 1: e / row_len == umul64hi(e, magic) while n * row_len < 2^64; 0: row_len 1
-    int row_len;              // 0: contiguous gradient
+    AwDivisor rows;           // of the gradient
     float neg_step, decay, bc2;   // -(lr / (1 - beta1^t)), 1 - lr wd, sqrt(1 - beta2^t) (8 bits: its reciprocal)
     float beta1, beta2, one_minus_beta1, one_minus_beta2, eps;
     uint32_t key;
@@ -87,36 +102,227 @@ __device__ __forceinline__ float aw_bf16(uint16_t b) { return __uint_as_float((u
 
 __device__ __forceinline__ float aw_level_m(uint32_t code, float scale) {
     const uint32_t c = code & 127u;
-    const float f = __uint_as_float(0x3F800000u - ((127u - c) << 20)) * scale;
-    return c == 0 ? 0.0f : (code & 128u) ? -f : f;
+    const float f = __uint_as_float((c << 20) + (0x3F800000u - (127u << 20))) * scale;
+    return c == 0 ? 0.0f : __uint_as_float(__float_as_uint(f) ^ (code & 128u) << 24);
 }
 __device__ __forceinline__ float aw_level_u(uint32_t code, float scale) {
-    const float f = __uint_as_float(0x3F800000u - ((255u - code) << 19)) * scale;
+    const float f = __uint_as_float((code << 19) + (0x3F800000u - (255u << 19))) * scale;
     return code == 0 ? 0.0f : f;
 }
-// x = the value over its block's scale, at most 1; r = 16 random bits, 32768 rounds to nearest
-__device__ __forceinline__ uint32_t aw_code_m(float x, bool negative, uint32_t r) {
-    int c = 127 + ((int)(__float_as_uint(x) + r * 16u - 0x3F800000u) >> 20);
-    if (c < 1) c = x * (65536.0f / (1.25f * 0x1p-16f)) > (float)r ? 1 : 0;
-    return (uint32_t)c + (negative && c > 0 ? 128u : 0u);
+// x = the value over its block's scale, at most 1 (also for NaN); r = 16 random bits, 32768 rounds to nearest
+__device__ __forceinline__ uint32_t aw_code_m(float x, uint32_t value_bits, uint32_t r) {
+    int c = (int)((r << 4) + __float_as_uint(x) - (0x3F800000u - (127u << 20))) >> 20;
+    const int lowest = x * (65536.0f / (1.25f * 0x1p-16f)) > (float)r ? 1 : 0;
+    c = c < 1 ? lowest : c;
+    return c == 0 ? 0u : (uint32_t)c | (value_bits >> 24 & 128u);
 }
-__device__ __forceinline__ uint32_t aw_code_u(float x, bool zero, uint32_t r) {
-    const int c = 255 + ((int)(__float_as_uint(x) + r * 8u - 0x3F800000u) >> 19);
-    return zero ? 0u : (uint32_t)(c < 1 ? 1 : c);
+__device__ __forceinline__ uint32_t aw_code_u(float x, uint32_t r) {
+    const int c = (int)((r << 3) + __float_as_uint(x) - (0x3F800000u - (255u << 19))) >> 19;
+    return x == 0.0f ? 0u : (uint32_t)(c < 1 ? 1 : c);
 }
 // the scale to keep and the factor that takes values to 0..1 (subnormal maxima count as zero: their reciprocal overflows)
 __device__ __forceinline__ float aw_scale(uint32_t max_bits, float& inverse) {
-    if (max_bits < 0x00800000u) { inverse = 0.0f; return 0.0f; }
-    inverse = __fdiv_rn(1.0f, __uint_as_float(max_bits));
-    return __uint_as_float(max_bits);
+    const float scale = max_bits < 0x00800000u ? 0.0f : __uint_as_float(max_bits);
+    const float x = __fdiv_rn(1.0f, scale);
+    inverse = max_bits < 0x00800000u ? 0.0f : x;
+    return scale;
 }
-__device__ __forceinline__ uint32_t aw_wave_max(uint32_t x) {
+// The largest of x over the 16 lanes of a DPP row, in all of them.
+__device__ __forceinline__ uint32_t aw_row_max(uint32_t x) {
+    uint32_t y;
+    y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, true); x = x > y ? x : y;   // row_ror:8
+    y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, true); x = x > y ? x : y;   // row_ror:4
+    y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xf, 0xf, true); x = x > y ? x : y;   // row_ror:2
+    y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xf, 0xf, true); x = x > y ? x : y;   // row_ror:1
+    return x;
+}
+
+// Four consecutive elements belong to a lane and a block of 64 to the 16 lanes of a DPP row: loads and stores are 16 bytes
+// wide (8 for 16-bit types and code pairs) and the block's maxima take four DPP steps, no LDS and no barrier.  The hardware
+// takes such accesses at any multiple of the element's size, so views need no form of their own.
+constexpr int AW_LANE = 4;
+constexpr int AW_ITERS = AW_CHUNK / (AW_THREADS * AW_LANE);
+static_assert(GS_ADAMW_BLOCK == 16 * AW_LANE && AW_CHUNK % (AW_THREADS * AW_LANE) == 0, "a DPP row holds a block");
+
+typedef float f4v __attribute__((ext_vector_type(4)));
+typedef uint32_t u2v __attribute__((ext_vector_type(2)));
+typedef float f4m __attribute__((ext_vector_type(4), aligned(4)));        // as they lie in memory
+typedef uint32_t u2m __attribute__((ext_vector_type(2), aligned(2)));
+
+// Codes of four elements: m[], u[] in, the pairs and the block's scales out.
+__device__ __forceinline__ u2v aw_pack4(const float* m, const float* u, const uint32_t* r, float& sm, float& su) {
+    uint32_t mm = 0, mu = 0;
 #pragma unroll
-    for (int d = 32; d; d >>= 1) {
-        const uint32_t y = (uint32_t)__shfl_xor((int)x, d, 64);
-        x = x > y ? x : y;
+    for (int c = 0; c < 4; ++c) {
+        const uint32_t bm = __float_as_uint(m[c]) & 0x7FFFFFFFu, bu = __float_as_uint(u[c]);
+        mm = mm > bm ? mm : bm;
+        mu = mu > bu ? mu : bu;
+    }
+    float im, iu;
+    sm = aw_scale(aw_row_max(mm), im);
+    su = aw_scale(aw_row_max(mu), iu);
+    uint32_t pair[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        pair[c] = aw_code_m(fminf(fabsf(m[c]) * im, 1.0f), __float_as_uint(m[c]), r[c] & 0xFFFFu) |
+                  aw_code_u(fminf(u[c] * iu, 1.0f), r[c] >> 16) << 8;
+    return u2v{pair[0] | pair[1] << 16, pair[2] | pair[3] << 16};
+}
+
+// how many of the four elements at `off` lie among the `left` ones
+__device__ __forceinline__ int aw_count(int off, int left) { return off >= left ? 0 : left - off < 4 ? left - off : 4; }
+// elements i .. i + 3 of a tensor, the first `count` of them (zeros for the rest)
+__device__ __forceinline__ f4v aw_load4(const float* p, int i, int count) {
+    f4v x{0.0f, 0.0f, 0.0f, 0.0f};
+    if (count == 4) x = *reinterpret_cast<const f4m*>(p + i);
+    else
+#pragma unroll
+        for (int c = 0; c < 3; ++c)
+            if (c < count) x[c] = p[i + c];
+    return x;
+}
+__device__ __forceinline__ u2v aw_load4(const uint16_t* p, int i, int count) {
+    u2v x{0, 0};
+    if (count == 4) x = *reinterpret_cast<const u2m*>(p + i);
+    else
+#pragma unroll
+        for (int c = 0; c < 3; ++c)
+            if (c < count) x[c / 2] |= (uint32_t)p[i + c] << (c % 2 * 16);
+    return x;
+}
+// Streamed once per call and mostly far larger than the caches: non-temporal, out of the way of the reads.
+__device__ __forceinline__ void aw_store4(float* p, int i, int count, f4v x) {
+    if (count == 4) __builtin_nontemporal_store(x, reinterpret_cast<f4m*>(p + i));
+    else
+#pragma unroll
+        for (int c = 0; c < 3; ++c)
+            if (c < count) p[i + c] = x[c];
+}
+__device__ __forceinline__ void aw_store4(uint16_t* p, int i, int count, u2v x) {
+    if (count == 4) __builtin_nontemporal_store(x, reinterpret_cast<u2m*>(p + i));
+    else
+#pragma unroll
+        for (int c = 0; c < 3; ++c)
+            if (c < count) p[i + c] = (uint16_t)(x[c / 2] >> (c % 2 * 16));
+}
+__device__ __forceinline__ uint32_t aw_half(u2v x, int c) { return x[c / 2] >> (c % 2 * 16) & 0xFFFFu; }
+
+// Four elements, `off` after the start of a chunk, of a matrix with a row stride.  Lanes whose elements lie in one row take them at once.
+template <class Element>
+__device__ __forceinline__ auto aw_load4_rows(const Element* p, long long base, int off, int count, const AwRows& r, long long stride) {
+    if (r.len == 0) return aw_load4(p + base, off, count);
+    AwPlace at = aw_place(r, (uint32_t)off);
+    const Element* row = p + (r.row + at.q) * stride;
+    if (at.col + 4 <= r.len) return aw_load4(row, at.col, count);
+    decltype(aw_load4(p, 0, count)) x{};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        if (c < count) {
+            const Element y = row[at.col];
+            if constexpr (sizeof(Element) == 4) x[c] = y;
+            else x[c / 2] |= (uint32_t)y << (c % 2 * 16);
+        }
+        if (++at.col == r.len) { at.col = 0; row += stride; }
     }
     return x;
+}
+
+template <bool BF16> struct AwTypes { typedef f4v vec; typedef float element; };
+template <> struct AwTypes<true> { typedef u2v vec; typedef uint16_t element; };
+
+struct AwScalars { float neg_step, decay, bc2, coef; uint32_t key; bool clip; };
+
+// FAST: the whole chunk lies inside the tensor.
+template <bool BF16, bool Q8, bool FAST>
+__device__ __forceinline__ void adamw_chunk(const AwArgs& a, const AwTensor& T, const AwScalars& S, long long base) {
+    typedef typename AwTypes<BF16>::vec PVec;
+    typedef typename AwTypes<BF16>::element PElement;
+    PVec p4[AW_ITERS], g4[AW_ITERS];
+    u2v low4[AW_ITERS], codes[AW_ITERS];
+    f4v m4[AW_ITERS], v4[AW_ITERS];
+    float2 scale[AW_ITERS];
+    const AwRows rows = aw_rows(base, T.rows);
+    const int left = FAST ? AW_CHUNK : T.n - base < AW_CHUNK ? (int)(T.n - base) : AW_CHUNK;
+    PElement* const pp = (PElement*)T.p + base;
+    uint16_t* const pl = (uint16_t*)T.low + base;
+    uint16_t* const pc = (uint16_t*)T.m + base;           // 8 bits: the code pairs and scale pairs
+    float2* const ps = (float2*)T.v + base / GS_ADAMW_BLOCK;
+    float* const pm = (float*)T.m + base;                 // 32 bits: the moments
+    float* const pv = T.v + base;
+#pragma unroll
+    for (int i = 0; i < AW_ITERS; ++i) {
+        const int off = (i * AW_THREADS + (int)threadIdx.x) * AW_LANE;
+        const int count = FAST ? 4 : aw_count(off, left);
+        p4[i] = aw_load4(pp, off, count);
+        if (BF16) low4[i] = aw_load4(pl, off, count);
+        if (Q8) {
+            codes[i] = aw_load4(pc, off, count);
+            scale[i] = count > 0 ? ps[off / GS_ADAMW_BLOCK] : make_float2(0.0f, 0.0f);
+        } else {
+            m4[i] = aw_load4(pm, off, count);
+            v4[i] = aw_load4(pv, off, count);
+        }
+        g4[i] = aw_load4_rows((const PElement*)T.g, base, off, count, rows, T.g_row_stride);
+    }
+#pragma unroll
+    for (int i = 0; i < AW_ITERS; ++i) {
+        const int off = (i * AW_THREADS + (int)threadIdx.x) * AW_LANE;
+        const int count = FAST ? 4 : aw_count(off, left);
+        float p[4], m[4], v[4], u[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            float g;
+            if constexpr (BF16) {
+                p[c] = aw_join((uint16_t)aw_half(p4[i], c), (int16_t)aw_half(low4[i], c));
+                g = aw_bf16((uint16_t)aw_half(g4[i], c));
+            } else {
+                p[c] = p4[i][c];
+                g = g4[i][c];
+            }
+            if (S.clip) g = g * S.coef;
+            p[c] = p[c] * S.decay;
+            if (Q8) {
+                const uint32_t pair = aw_half(codes[i], c);
+                const float x = aw_level_u(pair >> 8, scale[i].y);
+                m[c] = aw_level_m(pair & 255u, scale[i].x) * T.beta1 + g * T.one_minus_beta1;
+                v[c] = (x * x) * T.beta2 + (g * g) * T.one_minus_beta2;
+                u[c] = sqrtf(v[c]);
+                p[c] = p[c] + S.neg_step * __fdiv_rn(m[c], u[c] * S.bc2 + T.eps);
+            } else {
+                m[c] = __fmaf_rn(T.one_minus_beta1, g - m4[i][c], m4[i][c]);
+                v[c] = __fmaf_rn(T.one_minus_beta2, g * g, v4[i][c] * T.beta2);
+                u[c] = sqrtf(v[c]);
+                p[c] = __fmaf_rn(S.neg_step, __fdiv_rn(m[c], __fdiv_rn(u[c], S.bc2) + T.eps), p[c]);
+            }
+        }
+        if (Q8) {
+            uint32_t r[4];
+            // chunks do not cross a multiple of 2^32
+            const uint32_t seed = (uint32_t)base + S.key + (uint32_t)((unsigned long long)base >> 32) * 0x3C6EF373u + (uint32_t)off;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) r[c] = a.stochastic ? aw_mix(seed + c) : 0x80008000u;
+            float2 s;
+            aw_store4(pc, off, count, aw_pack4(m, u, r, s.x, s.y));      // past the end everything is 0
+            if (count > 0 && (threadIdx.x & 15) == 0) ps[off / GS_ADAMW_BLOCK] = s;
+        } else {
+            aw_store4(pm, off, count, f4v{m[0], m[1], m[2], m[3]});
+            aw_store4(pv, off, count, f4v{v[0], v[1], v[2], v[3]});
+        }
+        if constexpr (BF16) {
+            u2v h{0, 0}, l{0, 0};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint16_t high; int16_t low;
+                aw_split(p[c], high, low);
+                h[c / 2] |= (uint32_t)high << (c % 2 * 16);
+                l[c / 2] |= (uint32_t)(uint16_t)low << (c % 2 * 16);
+            }
+            aw_store4(pp, off, count, h);
+            aw_store4(pl, off, count, l);
+        } else {
+            aw_store4(pp, off, count, f4v{p[0], p[1], p[2], p[3]});
+        }
+    }
 }
 
 template <bool BF16, bool Q8>
@@ -124,80 +330,15 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_kernel(const AwArgs a) {
     int ti = 0;
     for (int k = 1; k < a.count; ++k) ti += blockIdx.x >= a.block_begin[k] ? 1 : 0;
     const AwTensor& T = a.t[ti];
-    float neg_step = T.neg_step, decay = T.decay, bc2 = T.bc2;
-    uint32_t key = T.key;
+    const long long base = (long long)(blockIdx.x - a.block_begin[ti]) * AW_CHUNK;
+    AwScalars S{T.neg_step, T.decay, T.bc2, 1.0f, T.key, a.grad_norm != nullptr};
     if (a.scalars) {
         const float4 s = a.scalars[ti];
-        neg_step = s.x; decay = s.y; bc2 = s.z; key = __float_as_uint(s.w);
+        S.neg_step = s.x; S.decay = s.y; S.bc2 = s.z; S.key = __float_as_uint(s.w);
     }
-    for (int i = 0; i < AW_CHUNK; i += AW_THREADS) {
-        const long long e = (long long)(blockIdx.x - a.block_begin[ti]) * AW_CHUNK + i + threadIdx.x;
-        const bool in = e < T.n;
-        float p = 0.0f, g = 0.0f, m = 0.0f, v = 0.0f;
-        if (in) {
-            long long ge = e;
-            if (T.row_len) {
-                const long long row = T.magic ? (long long)__umul64hi((unsigned long long)e, T.magic) : e;
-                ge = row * T.g_row_stride + (e - row * T.row_len);
-            }
-            if (BF16) {
-                p = aw_join(((const uint16_t*)T.p)[e], T.low[e]);
-                g = aw_bf16(((const uint16_t*)T.g)[ge]);
-            } else {
-                p = ((const float*)T.p)[e];
-                g = ((const float*)T.g)[ge];
-            }
-            if (Q8) {
-                const uint32_t codes = ((const uint16_t*)T.m)[e];
-                const float2 s = ((const float2*)T.v)[e / GS_ADAMW_BLOCK];
-                m = aw_level_m(codes & 255u, s.x);
-                const float u = aw_level_u(codes >> 8, s.y);
-                v = u * u;
-            } else {
-                m = ((const float*)T.m)[e];
-                v = T.v[e];
-            }
-            if (a.grad_norm) g = g * aw_coef(a.grad_norm, a.max_norm);
-        }
-        float u;
-        p = p * decay;
-        if (Q8) {
-            m = m * T.beta1 + g * T.one_minus_beta1;
-            v = v * T.beta2 + (g * g) * T.one_minus_beta2;
-            u = sqrtf(v);
-            p = p + neg_step * __fdiv_rn(m, u * bc2 + T.eps);
-        } else {
-            m = __fmaf_rn(T.one_minus_beta1, g - m, m);
-            v = __fmaf_rn(T.one_minus_beta2, g * g, v * T.beta2);
-            u = sqrtf(v);
-            p = __fmaf_rn(neg_step, __fdiv_rn(m, __fdiv_rn(u, bc2) + T.eps), p);
-        }
-        if (Q8) {
-            // one wave holds one block of 64; lanes past the end bring zeros
-            float im, iu;
-            const float sm = aw_scale(aw_wave_max(in ? __float_as_uint(m) & 0x7FFFFFFFu : 0u), im);
-            const float su = aw_scale(aw_wave_max(in ? __float_as_uint(u) : 0u), iu);
-            uint32_t r = 0x80008000u;
-            if (a.stochastic) r = aw_mix((uint32_t)e + key + (uint32_t)((unsigned long long)e >> 32) * 0x3C6EF373u);
-            const uint32_t cm = aw_code_m(fminf(fabsf(m) * im, 1.0f), m < 0.0f, r & 0xFFFFu);
-            const uint32_t cu = aw_code_u(fminf(u * iu, 1.0f), u == 0.0f || su == 0.0f, r >> 16);
-            if (in) {
-                ((uint16_t*)T.m)[e] = (uint16_t)(cm | cu << 8);
-                if ((threadIdx.x & 63) == 0) ((float2*)T.v)[e / GS_ADAMW_BLOCK] = make_float2(sm, su);
-            }
-        }
-        if (in) {
-            if (BF16) {
-                uint16_t high; int16_t low;
-                aw_split(p, high, low);
-                ((uint16_t*)T.p)[e] = high;
-                T.low[e] = low;
-            } else {
-                ((float*)T.p)[e] = p;
-            }
-            if (!Q8) { ((float*)T.m)[e] = m; T.v[e] = v; }
-        }
-    }
+    if (S.clip) S.coef = aw_coef(a.grad_norm, a.max_norm);
+    if (base + AW_CHUNK <= T.n) adamw_chunk<BF16, Q8, true>(a, T, S, base);
+    else adamw_chunk<BF16, Q8, false>(a, T, S, base);
 }
 
 // ---- counts and learning rates kept on the device (so that a captured step counts on when it is replayed) ----------
@@ -217,9 +358,17 @@ __global__ __launch_bounds__(64) void adamw_scalars_kernel(const AwScalarArgs a)
 }
 
 // ---- sum of squares over many tensors -------------------------------------------------------------------------------
-constexpr int NRM_MAX_TENSORS = 64;
-constexpr int NRM_CHUNK = 8192;         // elements per workgroup and partial sum
-struct NrmTensor { const void* g; long long n, row_stride; unsigned long long magic; int row_len; int bf16; };
+// The order of the elements is free, so a lane takes a group of four elements of one row (contiguous tensors are one row): group j
+// starts at element 4 j, or at the row's fourth from last, and then leaves out what the group before it has.  No load
+// crosses a row, none depends on another, and all eight of a lane are under way before the first use.
+constexpr int NRM_MAX_TENSORS = 48;
+constexpr int NRM_GROUPS = 2048;        // groups per workgroup and partial sum
+struct NrmTensor {
+    const void* g;
+    long long groups, row_stride, row_len;
+    AwDivisor per_row;                  // groups of a row; len 0: one row
+    int bf16;
+};
 struct NrmArgs { NrmTensor t[NRM_MAX_TENSORS]; uint32_t block_begin[NRM_MAX_TENSORS + 1]; int count; double* partial; };
 
 __device__ __forceinline__ double nrm_block_sum(double s, double* lds) {
@@ -234,25 +383,62 @@ __device__ __forceinline__ double nrm_block_sum(double s, double* lds) {
     return s;
 }
 
+template <class Element>
+__device__ __forceinline__ double nrm_chunk(const NrmTensor& T, long long base) {
+    constexpr int ITERS = NRM_GROUPS / AW_THREADS;
+    decltype(aw_load4((const Element*)nullptr, 0, 4)) x[ITERS];
+    int skip[ITERS];                    // elements of the group that do not count
+    const AwRows rows = aw_rows(base, T.per_row);
+    const int last = T.groups - base < NRM_GROUPS ? (int)(T.groups - base) - 1 : NRM_GROUPS - 1;
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) {
+        const int off = i * AW_THREADS + (int)threadIdx.x, o = off < last ? off : last;
+        const Element* p;
+        if (T.per_row.len == 0) {
+            const long long over = 4 * (base + o) - (T.row_len - 4);
+            skip[i] = over > 0 ? (int)over : 0;
+            p = (const Element*)T.g + 4 * base + (4 * o - skip[i]);
+        } else {
+            const AwPlace at = aw_place(rows, (uint32_t)o);
+            const int over = (int)(4 * at.col) - ((int)T.row_len - 4);
+            skip[i] = over > 0 ? over : 0;
+            p = (const Element*)T.g + (rows.row + at.q) * T.row_stride + (4 * (int)at.col - skip[i]);
+        }
+        if (T.row_len >= 4) {
+            x[i] = aw_load4(p, 0, 4);
+        } else {                        // the row's elements sit in the places that count
+            x[i] = {};
+#pragma unroll
+            for (int c = 1; c < 4; ++c)
+                if (c >= 4 - T.row_len) {
+                    if constexpr (sizeof(Element) == 4) x[i][c] = p[c];
+                    else x[i][c / 2] |= (uint32_t)p[c] << (c % 2 * 16);
+                }
+        }
+        if (off > last) skip[i] = 4;
+    }
+    double s0 = 0.0, s1 = 0.0;          // two sums, so that the additions of a lane do not wait for each other
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            float y;
+            if constexpr (sizeof(Element) == 4) y = x[i][c];
+            else y = aw_bf16((uint16_t)aw_half(x[i], c));
+            const double z = c < skip[i] ? 0.0f : y;
+            if (c & 1) s1 = fma(z, z, s1);
+            else s0 = fma(z, z, s0);
+        }
+    return s0 + s1;
+}
+
 __global__ __launch_bounds__(AW_THREADS) void grad_norm_partial_kernel(const NrmArgs a) {
     __shared__ double lds[AW_THREADS / 64];
     int ti = 0;
     for (int k = 1; k < a.count; ++k) ti += blockIdx.x >= a.block_begin[k] ? 1 : 0;
     const NrmTensor& T = a.t[ti];
-    const long long base = (long long)(blockIdx.x - a.block_begin[ti]) * NRM_CHUNK;
-    double s = 0.0;
-    for (int k = 0; k < NRM_CHUNK; k += AW_THREADS) {
-        const long long e = base + k + threadIdx.x;
-        if (e < T.n) {
-            long long ge = e;
-            if (T.row_len) {
-                const long long row = T.magic ? (long long)__umul64hi((unsigned long long)e, T.magic) : e;
-                ge = row * T.row_stride + (e - row * T.row_len);
-            }
-            const double x = T.bf16 ? (double)aw_bf16(((const uint16_t*)T.g)[ge]) : (double)((const float*)T.g)[ge];
-            s = fma(x, x, s);
-        }
-    }
+    const long long base = (long long)(blockIdx.x - a.block_begin[ti]) * NRM_GROUPS;
+    double s = T.bf16 ? nrm_chunk<uint16_t>(T, base) : nrm_chunk<float>(T, base);
     s = nrm_block_sum(s, lds);
     if (threadIdx.x == 0) a.partial[blockIdx.x] = s;
 }
@@ -271,54 +457,185 @@ struct RowTensor {
     const void* src_m; const float* src_v; const int16_t* src_low;
     void* dst_m; float* dst_v; int16_t* dst_low;
     long long n;                          // elements of the new state
-    unsigned long long magic;
-    int row_len; int pad;
+    AwDivisor rows;
 };
 struct RowArgs { RowTensor t[AW_MAX_TENSORS]; uint32_t block_begin[AW_MAX_TENSORS + 1]; int count; long long src_rows; const int64_t* index; };
+
+__device__ __forceinline__ bool rows_valid(const RowArgs& a, long long row) { return row >= 0 && row < a.src_rows; }
+
+// x[c] = (lo, hi)[c + shift], shift 0..3
+__device__ __forceinline__ f4v rows_window(f4v lo, f4v hi, int shift) {
+    float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+    for (int c = 0; c < 6; ++c) x[c] = shift & 1 ? x[c + 1] : x[c];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) x[c] = shift & 2 ? x[c + 2] : x[c];
+    return f4v{x[0], x[1], x[2], x[3]};
+}
+__device__ __forceinline__ u2v rows_window(u2v lo, u2v hi, int shift) {
+    const uint64_t l = lo[0] | (uint64_t)lo[1] << 32, h = hi[0] | (uint64_t)hi[1] << 32;
+    const uint64_t x = shift ? l >> (16 * shift) | h << (64 - 16 * shift) : l;
+    return u2v{(uint32_t)x, (uint32_t)(x >> 32)};
+}
+
+template <bool Q8>
+__device__ __forceinline__ void rows_store(const RowTensor& T, long long base, int off, int count, f4v m, f4v v, u2v low) {
+    if (Q8) {
+        const uint32_t r[4] = {0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
+        const float mm[4] = {m[0], m[1], m[2], m[3]}, uu[4] = {v[0], v[1], v[2], v[3]};
+        float2 s;
+        aw_store4((uint16_t*)T.dst_m + base, off, count, aw_pack4(mm, uu, r, s.x, s.y));
+        if (count > 0 && (threadIdx.x & 15) == 0) ((float2*)T.dst_v)[base / GS_ADAMW_BLOCK + off / GS_ADAMW_BLOCK] = s;
+    } else {
+        aw_store4((float*)T.dst_m + base, off, count, m);
+        aw_store4(T.dst_v + base, off, count, v);
+    }
+    if (T.dst_low) aw_store4((uint16_t*)T.dst_low + base, off, count, low);
+}
+
+// Rows of four elements and more: a lane's four elements lie in one row or in two.  It loads four elements of the first row (the row's
+// last four if they end there) and, if needed, the first four of the second, and shifts them together: no load
+// depends on another but on the index.  Every phase runs for all of the lane's groups before the next one, so that the loads overlap.
+template <bool Q8>
+__device__ __forceinline__ void rows_long(const RowArgs& a, const RowTensor& T, long long base) {
+    const AwRows rows = aw_rows(base, T.rows);
+    const int left = T.n - base < AW_CHUNK ? (int)(T.n - base) : AW_CHUNK;
+    const int64_t* const index = a.index + rows.row;
+    long long k0[AW_ITERS], k1[AW_ITERS];     // first the rows, then where the lane's elements of the first and second row start in the source
+    int shift[AW_ITERS];
+    uint32_t col[AW_ITERS];
+#pragma unroll
+    for (int i = 0; i < AW_ITERS; ++i) {
+        const int off = (i * AW_THREADS + (int)threadIdx.x) * AW_LANE;
+        const AwPlace at = aw_place(rows, (uint32_t)off);
+        const int over = (int)(at.col + 4 - rows.len);    // elements in the second row
+        shift[i] = over > 0 ? over : 0;
+        col[i] = at.col - shift[i];
+        k0[i] = k1[i] = -1;
+        if (off < left) k0[i] = index[at.q];
+        if (over > 0 && off + 4 - over < left) k1[i] = index[at.q + 1];
+    }
+    u2v p0[AW_ITERS], p1[AW_ITERS], l0[AW_ITERS], l1[AW_ITERS];
+    f4v m0[AW_ITERS], m1[AW_ITERS], v0[AW_ITERS], v1[AW_ITERS];
+    float2 s00[AW_ITERS], s01[AW_ITERS], s10[AW_ITERS], s11[AW_ITERS];
+#pragma unroll
+    for (int i = 0; i < AW_ITERS; ++i) {
+        p0[i] = p1[i] = l0[i] = l1[i] = u2v{0, 0};
+        m0[i] = m1[i] = v0[i] = v1[i] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+        s00[i] = s01[i] = s10[i] = s11[i] = make_float2(0.0f, 0.0f);
+        if (rows_valid(a, k0[i])) {
+            const long long k = k0[i] = k0[i] * rows.len + col[i];
+            if (Q8) {
+                p0[i] = aw_load4((const uint16_t*)T.src_m + k, 0, 4);
+                s00[i] = ((const float2*)T.src_v)[k / GS_ADAMW_BLOCK];
+                s01[i] = ((const float2*)T.src_v)[(k + 3) / GS_ADAMW_BLOCK];
+            } else {
+                m0[i] = aw_load4((const float*)T.src_m + k, 0, 4);
+                v0[i] = aw_load4(T.src_v + k, 0, 4);
+            }
+            if (T.src_low) l0[i] = aw_load4((const uint16_t*)T.src_low + k, 0, 4);
+        }
+        if (rows_valid(a, k1[i])) {
+            const long long k = k1[i] = k1[i] * rows.len;
+            if (Q8) {
+                p1[i] = aw_load4((const uint16_t*)T.src_m + k, 0, 4);
+                s10[i] = ((const float2*)T.src_v)[k / GS_ADAMW_BLOCK];
+                s11[i] = ((const float2*)T.src_v)[(k + 3) / GS_ADAMW_BLOCK];
+            } else {
+                m1[i] = aw_load4((const float*)T.src_m + k, 0, 4);
+                v1[i] = aw_load4(T.src_v + k, 0, 4);
+            }
+            if (T.src_low) l1[i] = aw_load4((const uint16_t*)T.src_low + k, 0, 4);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < AW_ITERS; ++i) {
+        const int off = (i * AW_THREADS + (int)threadIdx.x) * AW_LANE;
+        f4v m, v;
+        if (Q8) {
+            const u2v pairs = rows_window(p0[i], p1[i], shift[i]);
+            // the place of the first element that belongs to the second of the two blocks, seen from the group's first element
+            const int second0 = GS_ADAMW_BLOCK - (int)(k0[i] & (GS_ADAMW_BLOCK - 1)) - shift[i];
+            const int first1 = 4 - shift[i], second1 = first1 + GS_ADAMW_BLOCK - (int)(k1[i] & (GS_ADAMW_BLOCK - 1));
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float2 s = c < first1 ? (c < second0 ? s00[i] : s01[i]) : (c < second1 ? s10[i] : s11[i]);
+                m[c] = aw_level_m(aw_half(pairs, c) & 255u, s.x);
+                v[c] = aw_level_u(aw_half(pairs, c) >> 8, s.y);
+            }
+        } else {
+            m = rows_window(m0[i], m1[i], shift[i]);
+            v = rows_window(v0[i], v1[i], shift[i]);
+        }
+        rows_store<Q8>(T, base, off, aw_count(off, left), m, v, rows_window(l0[i], l1[i], shift[i]));
+    }
+}
+
+// Rows of one to three elements: one by one, again in phases.
+template <bool Q8>
+__device__ __forceinline__ void rows_short(const RowArgs& a, const RowTensor& T, long long base) {
+    const AwRows rows = aw_rows(base, T.rows);
+    const int left = T.n - base < AW_CHUNK ? (int)(T.n - base) : AW_CHUNK;
+    const int64_t* const index = a.index + rows.row;
+    long long k[AW_ITERS][4];
+#pragma unroll
+    for (int i = 0; i < AW_ITERS; ++i) {
+        const int off = (i * AW_THREADS + (int)threadIdx.x) * AW_LANE;
+        AwPlace at = aw_place(rows, (uint32_t)off);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            k[i][c] = off + c < left ? index[at.q] : -1;
+            if (++at.col == rows.len) { at.col = 0; ++at.q; }
+        }
+    }
+    uint32_t pair[AW_ITERS][4];
+    float2 s[AW_ITERS][4];
+    f4v m[AW_ITERS], v[AW_ITERS];
+    u2v low[AW_ITERS];
+#pragma unroll
+    for (int i = 0; i < AW_ITERS; ++i) {
+        uint32_t col = aw_place(rows, (uint32_t)((i * AW_THREADS + (int)threadIdx.x) * AW_LANE)).col;
+        low[i] = u2v{0, 0};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            pair[i][c] = 0;
+            s[i][c] = make_float2(0.0f, 0.0f);
+            m[i][c] = v[i][c] = 0.0f;
+            if (rows_valid(a, k[i][c])) {
+                const long long j = k[i][c] * rows.len + col;
+                if (Q8) {
+                    pair[i][c] = ((const uint16_t*)T.src_m)[j];
+                    s[i][c] = ((const float2*)T.src_v)[j / GS_ADAMW_BLOCK];
+                } else {
+                    m[i][c] = ((const float*)T.src_m)[j];
+                    v[i][c] = T.src_v[j];
+                }
+                if (T.src_low) low[i][c / 2] |= (uint32_t)(uint16_t)T.src_low[j] << (c % 2 * 16);
+            }
+            if (++col == rows.len) col = 0;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < AW_ITERS; ++i) {
+        const int off = (i * AW_THREADS + (int)threadIdx.x) * AW_LANE;
+        if (Q8)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                m[i][c] = aw_level_m(pair[i][c] & 255u, s[i][c].x);
+                v[i][c] = aw_level_u(pair[i][c] >> 8, s[i][c].y);
+            }
+        rows_store<Q8>(T, base, off, aw_count(off, left), m[i], v[i], low[i]);
+    }
+}
 
 template <bool Q8>
 __global__ __launch_bounds__(AW_THREADS) void adamw_rows_kernel(const RowArgs a) {
     int ti = 0;
     for (int k = 1; k < a.count; ++k) ti += blockIdx.x >= a.block_begin[k] ? 1 : 0;
     const RowTensor& T = a.t[ti];
-    for (int i = 0; i < AW_CHUNK; i += AW_THREADS) {
-        const long long e = (long long)(blockIdx.x - a.block_begin[ti]) * AW_CHUNK + i + threadIdx.x;
-        const bool in = e < T.n;
-        float m = 0.0f, v = 0.0f;             // Q8: v holds u
-        int16_t low = 0;
-        if (in) {
-            const long long row = T.magic ? (long long)__umul64hi((unsigned long long)e, T.magic) : e;
-            const long long src_row = a.index[row];
-            if (src_row >= 0 && src_row < a.src_rows) {
-                const long long s = src_row * T.row_len + (e - row * T.row_len);
-                if (Q8) {
-                    const uint32_t codes = ((const uint16_t*)T.src_m)[s];
-                    const float2 sc = ((const float2*)T.src_v)[s / GS_ADAMW_BLOCK];
-                    m = aw_level_m(codes & 255u, sc.x);
-                    v = aw_level_u(codes >> 8, sc.y);
-                } else {
-                    m = ((const float*)T.src_m)[s];
-                    v = T.src_v[s];
-                }
-                if (T.src_low) low = T.src_low[s];
-            }
-        }
-        if (Q8) {
-            float im, iu;
-            const float sm = aw_scale(aw_wave_max(__float_as_uint(m) & 0x7FFFFFFFu), im);
-            const float su = aw_scale(aw_wave_max(__float_as_uint(v)), iu);
-            const uint32_t cm = aw_code_m(fminf(fabsf(m) * im, 1.0f), m < 0.0f, 32768u);
-            const uint32_t cu = aw_code_u(fminf(v * iu, 1.0f), v == 0.0f || su == 0.0f, 32768u);
-            if (in) {
-                ((uint16_t*)T.dst_m)[e] = (uint16_t)(cm | cu << 8);
-                if ((threadIdx.x & 63) == 0) ((float2*)T.dst_v)[e / GS_ADAMW_BLOCK] = make_float2(sm, su);
-            }
-        } else if (in) {
-            ((float*)T.dst_m)[e] = m;
-            T.dst_v[e] = v;
-        }
-        if (in && T.dst_low) T.dst_low[e] = low;
-    }
+    const long long base = (long long)(blockIdx.x - a.block_begin[ti]) * AW_CHUNK;
+    if (T.rows.len >= 4) rows_long<Q8>(a, T, base);
+    else rows_short<Q8>(a, T, base);
 }
 
 // ---- what packed states and split parameters stand for --------------------------------------------------------------
@@ -329,17 +646,33 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_unpack_kernel(const UnpackAr
     int ti = 0;
     for (int k = 1; k < a.count; ++k) ti += blockIdx.x >= a.block_begin[k] ? 1 : 0;
     const UnpackTensor& T = a.t[ti];
-    for (int i = 0; i < AW_CHUNK; i += AW_THREADS) {
-        const long long e = (long long)(blockIdx.x - a.block_begin[ti]) * AW_CHUNK + i + threadIdx.x;
-        if (e >= T.n) return;
+    const long long base = (long long)(blockIdx.x - a.block_begin[ti]) * AW_CHUNK;
+    const int left = T.n - base < AW_CHUNK ? (int)(T.n - base) : AW_CHUNK;
+#pragma unroll
+    for (int i = 0; i < AW_ITERS; ++i) {
+        const int off = (i * AW_THREADS + (int)threadIdx.x) * AW_LANE;
+        if (off >= left) return;
+        const int count = aw_count(off, left);
         if (T.codes) {
-            const uint32_t codes = T.codes[e];
-            const float2 s = T.scales[e / GS_ADAMW_BLOCK];
-            const float u = aw_level_u(codes >> 8, s.y);
-            T.m[e] = aw_level_m(codes & 255u, s.x);
-            T.v[e] = u * u;
+            const float2 s = T.scales[base / GS_ADAMW_BLOCK + off / GS_ADAMW_BLOCK];
+            const u2v pairs = aw_load4(T.codes + base, off, count);
+            f4v m, v;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float u = aw_level_u(aw_half(pairs, c) >> 8, s.y);
+                m[c] = aw_level_m(aw_half(pairs, c) & 255u, s.x);
+                v[c] = u * u;
+            }
+            aw_store4(T.m + base, off, count, m);
+            aw_store4(T.v + base, off, count, v);
         }
-        if (T.p) T.x[e] = aw_join(T.p[e], T.low[e]);
+        if (T.p) {
+            const u2v h = aw_load4(T.p + base, off, count), l = aw_load4((const uint16_t*)T.low + base, off, count);
+            f4v x;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) x[c] = aw_join((uint16_t)aw_half(h, c), (int16_t)aw_half(l, c));
+            aw_store4(T.x + base, off, count, x);
+        }
     }
 }
 
@@ -349,7 +682,10 @@ bool aw_shape(long long rows, int row_len, long long& n) {
     n = rows * row_len;
     return true;
 }
-unsigned long long aw_magic(int row_len) { return row_len == 1 ? 0ull : ~0ull / (unsigned long long)row_len + 1ull; }
+AwDivisor aw_divisor(int len) {
+    if (len < 2) return AwDivisor{0, (uint32_t)len, 0};
+    return AwDivisor{~0ull / (unsigned long long)len + 1ull, (uint32_t)len, ~0u / (uint32_t)len + 1u};
+}
 
 // Gives the tensors of a launch their workgroups; false if the launch would need 2^32 threads (a grid's size is kept in 32 bits).
 template <class Args, class Size>
@@ -404,8 +740,7 @@ extern "C" int gs_adamw_step(int num_tensors, const GsAdamWTensor* tensors, int 
             d.p = s.param; d.g = s.grad; d.low = param_bf16 ? s.param_low : nullptr; d.m = s.exp_avg; d.v = s.exp_avg_sq;
             d.n = s.rows * s.row_len;
             d.g_row_stride = s.grad_row_stride ? s.grad_row_stride : s.row_len;
-            d.row_len = d.g_row_stride == s.row_len ? 0 : s.row_len;
-            d.magic = aw_magic(s.row_len);
+            d.rows = aw_divisor(d.g_row_stride == s.row_len ? 0 : s.row_len);
             // torch/optim/adam.py: Python doubles, rounded to fp32 when they meet the tensor
             const double root = sqrt(1.0 - pow(s.beta2, (double)s.step));
             d.neg_step = (float)(-(s.lr / (1.0 - pow(s.beta1, (double)s.step))));
@@ -440,7 +775,13 @@ extern "C" int gs_adamw_step(int num_tensors, const GsAdamWTensor* tensors, int 
     return GS_OK;
 }
 
-static long long nrm_blocks(const GsGradTensor& s) { return (s.rows * s.row_len + NRM_CHUNK - 1) / NRM_CHUNK; }
+// One row where the rows follow each other without a gap.
+static NrmTensor nrm_tensor(const GsGradTensor& s) {
+    const bool one = s.row_stride == 0 || s.row_stride == s.row_len;
+    const long long row_len = one ? s.rows * s.row_len : s.row_len, per_row = (row_len + 3) / 4;
+    return NrmTensor{s.grad, one ? per_row : s.rows * per_row, s.row_stride, row_len, aw_divisor(one ? 0 : (int)per_row), s.bf16};
+}
+static long long nrm_blocks(const GsGradTensor& s) { return (nrm_tensor(s).groups + NRM_GROUPS - 1) / NRM_GROUPS; }
 
 extern "C" size_t gs_grad_norm_workspace_bytes(int num_tensors, const GsGradTensor* tensors) {
     size_t blocks = 0;
@@ -467,14 +808,10 @@ extern "C" int gs_grad_norm(int num_tensors, const GsGradTensor* tensors, float*
     for (int first = 0; first < num_tensors; first += NRM_MAX_TENSORS) {
         const int count = num_tensors - first < NRM_MAX_TENSORS ? num_tensors - first : NRM_MAX_TENSORS;
         NrmArgs a{};
-        for (int k = 0; k < count; ++k) {
-            const GsGradTensor& s = tensors[first + k];
-            const long long stride = s.row_stride ? s.row_stride : s.row_len;
-            a.t[k] = NrmTensor{s.grad, s.rows * s.row_len, stride, aw_magic(s.row_len), stride == s.row_len ? 0 : s.row_len, s.bf16};
-        }
+        for (int k = 0; k < count; ++k) a.t[k] = nrm_tensor(tensors[first + k]);
         a.partial = (double*)workspace + done;
         uint32_t blocks = 0;
-        GS_REQUIRE(aw_plan(a, count, NRM_CHUNK, [&](int k) { return a.t[k].n; }, blocks), "too many workgroups");
+        GS_REQUIRE(aw_plan(a, count, NRM_GROUPS, [&](int k) { return a.t[k].groups; }, blocks), "too many workgroups");
         if (blocks == 0) continue;
         hipLaunchKernelGGL(grad_norm_partial_kernel, dim3(blocks), dim3(AW_THREADS), 0, (hipStream_t)stream_, a);
         GS_CHECK_LAUNCH("grad_norm_partial");
@@ -509,7 +846,7 @@ extern "C" int gs_adamw_gather_rows(int num_tensors, const GsAdamWRows* tensors,
             GS_REQUIRE((am & (q8 ? 1 : 3)) == 0 && (av & (q8 ? 7 : 3)) == 0 && (((uintptr_t)s.src_param_low | (uintptr_t)s.dst_param_low) & 1) == 0,
                        "tensor %d: misaligned pointer", first + k);
             a.t[k] = RowTensor{s.src_exp_avg, s.src_exp_avg_sq, s.src_param_low, s.dst_exp_avg, s.dst_exp_avg_sq, s.dst_param_low,
-                               n_dst, aw_magic(s.row_len), s.row_len, 0};
+                               n_dst, aw_divisor(s.row_len)};
         }
         uint32_t blocks = 0;
         GS_REQUIRE(aw_plan(a, count, AW_CHUNK, [&](int k) { return a.t[k].n; }, blocks), "too many workgroups");

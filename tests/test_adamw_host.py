@@ -43,7 +43,13 @@ def test_descriptor_structs_match_the_header(impl, adamw):
         assert int(out[n]) == C.sizeof(cls)
         for field, _ in cls._fields_:
             assert int(out[f"{n}.{field}"]) == getattr(cls, field).offset, (n, field)
-    assert adamw._STEP.size == C.sizeof(impl._lib.GsAdamWTensor) and adamw._GRAD.size == C.sizeof(impl._lib.GsGradTensor)
+    # the packed forms: every field in its place (a count up from 1 in the order of the struct)
+    for pack, cls in ((adamw._STEP, impl._lib.GsAdamWTensor), (adamw._GRAD, impl._lib.GsGradTensor), (adamw._ROWS, impl._lib.GsAdamWRows),
+                      (adamw._UNPACK, impl._lib.GsAdamWUnpack)):
+        packed = pack(*range(1, len(cls._fields_) + 1))
+        assert len(packed) == C.sizeof(cls)
+        got = cls.from_buffer_copy(packed)
+        assert [getattr(got, field) for field, _ in cls._fields_] == list(range(1, len(cls._fields_) + 1))
     assert impl._lib.load().gs_adamw_block() == adamw.BLOCK == orc.BLOCK
 
 
