@@ -66,6 +66,8 @@ struct AwTensor {
     float neg_step, decay, bc2;   // -(lr / (1 - beta1^t)), 1 - lr wd, sqrt(1 - beta2^t) (8 bits: its reciprocal)
     float beta1, beta2, one_minus_beta1, one_minus_beta2, eps;
     uint32_t key;
+    int slot;                 // place in `scalars`
+    uint32_t blocks, every;   // workgroups; > 0: `every` workgroups of the next tensor follow on each of this one's (see aw_pair)
 };
 
 struct AwArgs {
@@ -77,6 +79,8 @@ struct AwArgs {
     const float* grad_norm;   // or null
     float max_norm;
 };
+
+static_assert(sizeof(AwArgs) <= 4096, "kernel arguments");
 
 __host__ __device__ __forceinline__ uint32_t aw_mix(uint32_t x) {
     // two rounds of xor-shift and multiply (odd constants: fractional bits of sqrt(2) and sqrt(3))
@@ -329,11 +333,19 @@ template <bool BF16, bool Q8>
 __global__ __launch_bounds__(AW_THREADS) void adamw_kernel(const AwArgs a) {
     int ti = 0;
     for (int k = 1; k < a.count; ++k) ti += blockIdx.x >= a.block_begin[k] ? 1 : 0;
+    uint32_t block = blockIdx.x - a.block_begin[ti];
+    if (a.t[ti].every) {
+        const uint32_t every = a.t[ti].every, blocks = a.t[ti].blocks, group = block / (every + 1);
+        const uint32_t place = block - group * (every + 1);
+        if (group >= blocks) { block -= blocks; ++ti; }
+        else if (place > 0) { block = group * every + place - 1; ++ti; }
+        else block = group;
+    }
     const AwTensor& T = a.t[ti];
-    const long long base = (long long)(blockIdx.x - a.block_begin[ti]) * AW_CHUNK;
+    const long long base = (long long)block * AW_CHUNK;
     AwScalars S{T.neg_step, T.decay, T.bc2, 1.0f, T.key, a.grad_norm != nullptr};
     if (a.scalars) {
-        const float4 s = a.scalars[ti];
+        const float4 s = a.scalars[T.slot];
         S.neg_step = s.x; S.decay = s.y; S.bc2 = s.z; S.key = __float_as_uint(s.w);
     }
     if (S.clip) S.coef = aw_coef(a.grad_norm, a.max_norm);
@@ -702,6 +714,23 @@ bool aw_plan(Args& a, int count, int chunk, Size elements, uint32_t& blocks) {
     return true;
 }
 
+// Gradients that are column ranges of one matrix, as the rasterizer's colour gradients are for f_dc and f_rest (3 and 45 of 48
+// floats), share cache lines: one after the other, the narrow one would fetch nearly the whole matrix again (192-byte rows, 128-byte
+// lines: 384 MB for 36 MB at 3 M Gaussians).  Their workgroups alternate instead, in the ratio of their sizes, so that
+// a row's lines are fetched once and found in the cache by the other.
+bool aw_siblings(const AwTensor& x, const AwTensor& y, int size) {
+    if (!x.n || !x.rows.len || !y.rows.len || x.g_row_stride != y.g_row_stride || x.n / x.rows.len != y.n / y.rows.len) return false;
+    const long long apart = ((long long)(uintptr_t)y.g - (long long)(uintptr_t)x.g) / size;
+    return apart < x.g_row_stride && -apart < x.g_row_stride;
+}
+void aw_pair(AwArgs& a, int k) {          // tensors k and k + 1: their workgroups become k's
+    if (a.t[k].n > a.t[k + 1].n) { const AwTensor t = a.t[k]; a.t[k] = a.t[k + 1]; a.t[k + 1] = t; }
+    AwTensor& x = a.t[k];
+    x.blocks = (uint32_t)((x.n + AW_CHUNK - 1) / AW_CHUNK);
+    x.every = (uint32_t)((a.t[k + 1].n + AW_CHUNK - 1) / AW_CHUNK) / x.blocks;
+    a.block_begin[k + 1] = a.block_begin[k + 2];
+}
+
 }  // namespace
 
 extern "C" int gs_adamw_block(void) { return GS_ADAMW_BLOCK; }
@@ -751,6 +780,7 @@ extern "C" int gs_adamw_step(int num_tensors, const GsAdamWTensor* tensors, int 
             d.eps = (float)s.eps;
             const uint32_t seed = aw_mix(s.seed + 0x9E3779B9u * (s.index + 1u));
             d.key = aw_mix(seed ^ (uint32_t)s.step);
+            d.slot = k;
             sc.t[k] = AwScalarTensor{s.step_dev, s.lr_dev, s.lr, s.beta1, s.beta2, s.weight_decay, seed, 0};
         }
         a.stochastic = stochastic_rounding;
@@ -767,6 +797,8 @@ extern "C" int gs_adamw_step(int num_tensors, const GsAdamWTensor* tensors, int 
         uint32_t blocks = 0;
         GS_REQUIRE(aw_plan(a, count, AW_CHUNK, [&](int k) { return a.t[k].n; }, blocks), "too many workgroups");
         if (blocks == 0) continue;
+        for (int k = 0; k + 1 < count; ++k)
+            if (aw_siblings(a.t[k], a.t[k + 1], param_bf16 ? 2 : 4)) { aw_pair(a, k); ++k; }
         void (*kernel)(AwArgs) = param_bf16 ? (q8 ? adamw_kernel<true, true> : adamw_kernel<true, false>)
                                             : (q8 ? adamw_kernel<false, true> : adamw_kernel<false, false>);
         hipLaunchKernelGGL(kernel, dim3(blocks), dim3(AW_THREADS), 0, (hipStream_t)stream_, a);
@@ -775,6 +807,8 @@ extern "C" int gs_adamw_step(int num_tensors, const GsAdamWTensor* tensors, int 
     return GS_OK;
 }
 
+static_assert(sizeof(NrmArgs) <= 4096, "kernel arguments");
+
 // One row where the rows follow each other without a gap.
 static NrmTensor nrm_tensor(const GsGradTensor& s) {
     const bool one = s.row_stride == 0 || s.row_stride == s.row_len;
@@ -782,6 +816,22 @@ static NrmTensor nrm_tensor(const GsGradTensor& s) {
     return NrmTensor{s.grad, one ? per_row : s.rows * per_row, s.row_stride, row_len, aw_divisor(one ? 0 : (int)per_row), s.bf16};
 }
 static long long nrm_blocks(const GsGradTensor& s) { return (nrm_tensor(s).groups + NRM_GROUPS - 1) / NRM_GROUPS; }
+
+// Takes tensor k, and with it those after it that continue its rows: neighbouring column ranges of one matrix are read as one (f_dc
+// and f_rest of the rasterizer's colour gradient: 3 + 45 of 48 floats, and no line is fetched twice).  Returns how many it took.
+static int nrm_take(int num_tensors, const GsGradTensor* tensors, int k, GsGradTensor& out) {
+    out = tensors[k];
+    int taken = 1;
+    for (; k + taken < num_tensors; ++taken) {
+        const GsGradTensor& s = tensors[k + taken];
+        const long long size = out.bf16 ? 2 : 4;
+        if (!out.rows || out.row_stride <= out.row_len || s.rows != out.rows || s.row_stride != out.row_stride || !s.bf16 != !out.bf16 ||
+            (uintptr_t)s.grad != (uintptr_t)out.grad + (uintptr_t)(out.row_len * size) || (long long)out.row_len + s.row_len > out.row_stride ||
+            (long long)out.row_len + s.row_len > 0x7FFFFFFFll) break;
+        out.row_len += s.row_len;
+    }
+    return taken;
+}
 
 extern "C" size_t gs_grad_norm_workspace_bytes(int num_tensors, const GsGradTensor* tensors) {
     size_t blocks = 0;
@@ -805,10 +855,14 @@ extern "C" int gs_grad_norm(int num_tensors, const GsGradTensor* tensors, float*
     GS_REQUIRE(workspace_bytes >= (size_t)total * sizeof(double) && (total == 0 || workspace), "workspace too small");
     GS_REQUIRE(((uintptr_t)workspace & 7) == 0, "workspace must be 8-byte aligned");
     long long done = 0;
-    for (int first = 0; first < num_tensors; first += NRM_MAX_TENSORS) {
-        const int count = num_tensors - first < NRM_MAX_TENSORS ? num_tensors - first : NRM_MAX_TENSORS;
+    for (int next = 0; next < num_tensors;) {
+        int count = 0;
         NrmArgs a{};
-        for (int k = 0; k < count; ++k) a.t[k] = nrm_tensor(tensors[first + k]);
+        for (; next < num_tensors && count < NRM_MAX_TENSORS; ++count) {
+            GsGradTensor s;
+            next += nrm_take(num_tensors, tensors, next, s);
+            a.t[count] = nrm_tensor(s);
+        }
         a.partial = (double*)workspace + done;
         uint32_t blocks = 0;
         GS_REQUIRE(aw_plan(a, count, NRM_GROUPS, [&](int k) { return a.t[k].groups; }, blocks), "too many workgroups");

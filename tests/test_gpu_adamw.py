@@ -778,3 +778,50 @@ def test_training_loop_with_densification(impl, dev, bits):
     other = impl.FusedAdamW(groups({k: torch.nn.Parameter(p.detach().clone()) for k, p in params.items()}), lr=0.0, state_bits=bits)
     other.load_state_dict(sd)
     assert float(other.state[other.param_groups[0]["params"][0]]["step"]) == 6
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [1, 2, 43, 1000, 70_001])
+@pytest.mark.parametrize("cuts", [(1, 3, 48), (3, 48), (45, 48), (5, 9, 20, 41), (24, 48)])
+def test_column_ranges_of_one_matrix(impl, dev, n, cuts, dtype, bits):
+    """Gradients that are neighbouring column ranges of one (n, 48) matrix (their workgroups alternate, the norm reads them as one),
+    in both orders and with a gap: the same bits as from copies."""
+    gen = torch.Generator().manual_seed(n)
+    matrix = torch.randn(n, 48, generator=gen).to(dev, dtype)
+    edges = [0, *cuts]
+    ranges = list(zip(edges, edges[1:]))
+    for order in (ranges, ranges[::-1], ranges[::2]):
+        results = []
+        for copy in (False, True):
+            params = [torch.nn.Parameter(torch.ones(n, b - a, device=dev, dtype=dtype)) for a, b in order]
+            for p, (a, b) in zip(params, order):
+                p.grad = matrix[:, a:b].contiguous() if copy else matrix[:, a:b]
+            opt = impl.FusedAdamW(params, lr=0.01, state_bits=bits, seed=3)
+            for _ in range(2):
+                opt.step(max_norm=1.0)
+            results.append((params, opt))
+        (pa, oa), (pb, ob) = results
+        exact = math.sqrt(sum(float(p.grad.double().square().sum()) for p in pb))
+        for o in (oa, ob):
+            assert abs(float(o.last_grad_norm) - exact) <= 1.001 * E * exact
+        if torch.equal(oa.last_grad_norm, ob.last_grad_norm):        # fp64 sums of another order may round to either neighbour
+            for p, q in zip(pa, pb):
+                assert torch.equal(p, q)
+                for name, x in oa.state[p].items():
+                    assert torch.equal(x, ob.state[q][name]), name
+
+
+def test_column_ranges_in_a_captured_step(impl, dev):
+    """Counts on the device together with alternating workgroups: every tensor finds its own scalars."""
+    matrix = torch.randn(3000, 48, generator=torch.Generator().manual_seed(0)).to(dev)
+    runs = []
+    for capturable in (False, True):
+        params = [torch.nn.Parameter(torch.ones(3000, w, device=dev)) for w in (45, 3)]
+        params[0].grad, params[1].grad = matrix[:, 3:], matrix[:, :3]
+        opt = impl.FusedAdamW([{"params": [params[0]], "lr": 0.5}, {"params": [params[1]], "lr": 0.001}], capturable=capturable)
+        for _ in range(3):
+            opt.step()
+        runs.append(params)
+    for p, q in zip(*runs):
+        assert torch.equal(p, q)
