@@ -27,6 +27,8 @@ from .profiling import stage as _stage
 BLOCK = 64                                       # GS_ADAMW_BLOCK: elements that share a pair of scales
 _F32, _BF16 = torch.float32, torch.bfloat16
 
+_stream = torch._C._cuda_getCurrentRawStream     # of a device index; torch.cuda.current_stream() takes 2.5 us to make its object
+
 # The descriptors of include/gsplat.h as packed bytes: a step describes every tensor anew, and a small model's step takes as long as that does.
 _STEP = struct.Struct("@7P3q5diIIi").pack        # GsAdamWTensor
 _GRAD = struct.Struct("@P2q2i").pack             # GsGradTensor
@@ -48,10 +50,6 @@ class _On:
     def __exit__(self, *exc):
         if self.ctx is not None:
             self.ctx.__exit__(*exc)
-
-
-def _stream():
-    return torch.cuda.current_stream().cuda_stream
 
 
 def _matrix(g):
@@ -103,7 +101,7 @@ def grad_norm(grads):
         if g.device != dev:
             raise RuntimeError("grad_norm: all gradients must live on one device")
     with _On(dev), _stage("grad_norm"):
-        return _norm([_matrix(g) for g in grads], dev, _stream())
+        return _norm([_matrix(g) for g in grads], dev, _stream(dev.index))
 
 
 class FusedAdamW(torch.optim.AdamW):
@@ -165,7 +163,7 @@ class FusedAdamW(torch.optim.AdamW):
         with _On(dev), _stage("adamw"):
             if torch.cuda.is_current_stream_capturing():
                 self._check_capture(work)
-            stream = _stream()
+            stream = _stream(dev.index)
             mats = [_matrix(w[3]) for w in work]
             if max_norm is not None and grad_norm is None:
                 grad_norm = _norm(mats, dev, stream)
@@ -361,7 +359,7 @@ class FusedAdamW(torch.optim.AdamW):
         with _On(dev), _stage("adamw_rows"):
             index = index.contiguous()
             for bits, rows in buckets.items():
-                _lib.check(lib.gs_adamw_gather_rows(len(rows), b"".join(rows), bits, n, m, index.data_ptr(), _stream()), "gs_adamw_gather_rows")
+                _lib.check(lib.gs_adamw_gather_rows(len(rows), b"".join(rows), bits, n, m, index.data_ptr(), _stream(dev.index)), "gs_adamw_gather_rows")
         return out
 
     def replace_params(self, old, new, index):
@@ -439,7 +437,7 @@ class FusedAdamW(torch.optim.AdamW):
                 packed.append(_UNPACK(*entry, numel))
         if packed:
             with _On(dev), _stage("adamw_unpack"):
-                _lib.check(_lib.load().gs_adamw_unpack(len(packed), b"".join(packed), _stream()), "gs_adamw_unpack")
+                _lib.check(_lib.load().gs_adamw_unpack(len(packed), b"".join(packed), _stream(dev.index)), "gs_adamw_unpack")
         return out
 
     # ---- checkpoints --------------------------------------------------------------------------------------------------
