@@ -120,22 +120,22 @@ class FusedAdamW(torch.optim.AdamW):
             kw.pop(k, None)
         super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, amsgrad=False, foreach=False,
                          capturable=capturable, **kw)
-        self._own_defaults = {"state_bits": state_bits, "stochastic_rounding": bool(stochastic_rounding), "seed": int(seed)}
-        self.defaults.update(self._own_defaults)
+        self.defaults.update(state_bits=state_bits, stochastic_rounding=bool(stochastic_rounding), seed=int(seed))
         for group in self.param_groups:
             self._complete(group)
-        self.last_grad_norm = None
+
+    last_grad_norm = None
 
     def _complete(self, group):
-        for k, v in self._own_defaults.items():
-            group.setdefault(k, v)
+        for k in ("state_bits", "stochastic_rounding", "seed"):
+            group.setdefault(k, self.defaults[k])
         if group["state_bits"] not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, not {group['state_bits']!r}")
 
     def add_param_group(self, param_group):
+        if "state_bits" in self.defaults:        # not yet while the base class adds the first groups
+            self._complete(param_group)
         super().add_param_group(param_group)
-        if hasattr(self, "_own_defaults"):       # not yet while the base class adds the first groups
-            self._complete(self.param_groups[-1])
 
     # ---- the step ---------------------------------------------------------------------------------------------------
     def step(self, closure=None, *, max_norm=None, grad_norm=None):
@@ -366,6 +366,8 @@ class FusedAdamW(torch.optim.AdamW):
         """Puts ``new[k]`` in the place of ``old[k]`` in its group, with the state of the rows ``index`` (see gather_state): the
         reference's _prune_optimizer and cat_tensors_to_optimizer (scene/gaussian_model.py:476-530) in one call."""
         old, new = list(old), list(new)
+        if not torch.is_tensor(index):
+            raise ValueError("index must be a 1-d int64 tensor (of a mask: mask.nonzero()[:, 0])")
         if len(old) != len(new) or len({id(p) for p in old}) != len(old) or len({id(p) for p in new}) != len(new):
             raise ValueError("replace_params: as many new parameters as old ones, each once")
         for p, q in zip(old, new):
@@ -451,7 +453,7 @@ class FusedAdamW(torch.optim.AdamW):
             state = state_dict["state"].get(i)
             if state and ("moment_codes" if b == 8 else "exp_avg") not in state:
                 raise ValueError(f"state_dict holds no states in {b} bits for parameter {i}")
-        super().load_state_dict(state_dict)
+        super().load_state_dict({**state_dict, "state": {}})
         for group in self.param_groups:
             self._complete(group)
         params = [(group, p) for group in self.param_groups for p in group["params"]]

@@ -24,9 +24,11 @@
 // nearest would swallow every time.  The random bits are a hash of (seed, tensor, update, element): no state, and the
 // same results whatever the launch looks like.
 //
+// A NaN makes its whole block NaN (its maximum is), loudly; an infinity leaves nothing of its block's other moments, which start over.
+//
 // bf16 parameters: p holds the fp32 value rounded to bf16 (halves away from zero), a 16-bit remainder in units of the
 // fp32's last place holds the rest, so value = (bits(p) << 16) + remainder.  It costs what an fp32 parameter costs, and a
-// parameter that was overwritten from outside is off by no more than half a bf16 step.
+// parameter that was overwritten from outside with a finite value is off by no more than half a bf16 step.
 #include "gsplat_common.h"
 #include "../../include/gsplat.h"
 #include <math.h>
@@ -98,8 +100,11 @@ __device__ __forceinline__ float aw_coef(const float* norm, float max_norm) {
     return c > 1.0f ? 1.0f : c;           // a NaN norm stays NaN
 }
 
+// aw_split() gives a zero no negative remainder; one that was left behind when the parameter was set to zero from outside would borrow
+// through the sign and make a NaN of it, and is dropped.
 __device__ __forceinline__ float aw_join(uint16_t high, int16_t low) {
-    return __uint_as_float(((uint32_t)high << 16) + (uint32_t)(int32_t)low);
+    const uint32_t h = (uint32_t)high << 16, x = h + (uint32_t)(int32_t)low;
+    return __uint_as_float((int32_t)(x ^ h) < 0 ? h : x);
 }
 __device__ __forceinline__ void aw_split(float x, uint16_t& high, int16_t& low) {
     const uint32_t b = x != x ? 0x7FC00000u : __float_as_uint(x);
@@ -756,10 +761,14 @@ extern "C" int gs_adamw_step(int num_tensors, const GsAdamWTensor* tensors, int 
     GS_REQUIRE(!grad_norm || max_norm >= 0.0, "max_norm must not be negative");
     GS_REQUIRE(((uintptr_t)scalars & 15) == 0, "scalars must be 16-byte aligned");
     const bool q8 = state_bits == 8;
+    long long threads = 0;
     for (int k = 0; k < num_tensors; ++k) {
         const GsAdamWTensor& s = tensors[k];
         long long n;
         GS_REQUIRE(aw_shape(s.rows, s.row_len, n), "tensor %d: bad shape %lld x %d", k, s.rows, s.row_len);
+        // of the launch that tensor k is in: refused before the first launch, so that a refused call changes nothing
+        threads = (k % AW_MAX_TENSORS ? threads : 0) + (n + aw_step_chunk(q8) - 1) / aw_step_chunk(q8) * AW_THREADS;
+        GS_REQUIRE(threads < (1ll << 32), "tensor %d: too many workgroups", k);
         GS_REQUIRE(n == 0 || (s.param && s.grad && s.exp_avg && s.exp_avg_sq), "tensor %d: null pointer", k);
         GS_REQUIRE(n == 0 || !param_bf16 || s.param_low, "tensor %d: bf16 parameters need param_low", k);
         GS_REQUIRE(s.grad_row_stride == 0 || s.grad_row_stride >= s.row_len, "tensor %d: grad_row_stride %lld < row_len %d", k,

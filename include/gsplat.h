@@ -327,7 +327,7 @@ int gs_adam_densify_step(int num_groups, const GsAdamGroup* groups, double beta1
  *                  scale * float_with_bits(0x3F800000 - (127 - c) * 2^20).  sqrt(v): c = 0 is 0, else
  *                  scale * float_with_bits(0x3F800000 - (255 - c) * 2^19).  stochastic_rounding != 0: a value between two
  *                  levels goes up with the probability of its place between them; the random bits are a hash of (seed,
- *                  index, t, element).  0: nearest.  A block that takes in a NaN reads as NaN wherever it is not 0.
+ *                  index, t, element).  0: nearest.  A block that takes in a NaN reads as NaN.
  *   param_bf16:    the fp32 value is (bits(param) << 16) + param_low; both are updated.  NULL for fp32 parameters.
  *   grad_norm:     device scalar or NULL; with it every gradient is multiplied by min(1, max_norm / (grad_norm + 1e-6)).
  *   t:             `step` (host, the count after this update) or, for calls that are captured and replayed, *step_dev (device,

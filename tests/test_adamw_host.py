@@ -96,6 +96,8 @@ def test_python_refusals(impl):
         opt.replace_params([p], [torch.nn.Parameter(torch.randn(5, 3))], index)
     with pytest.raises(ValueError, match="each once"):
         opt.replace_params([p, p], [q, torch.nn.Parameter(torch.randn(4, 3))], index)
+    with pytest.raises(ValueError, match="int64"):
+        opt.replace_params([p], [q], [0, 1, 2, 3])
     with pytest.raises(ValueError, match="not both"):
         opt.unpacked([p], states=[])
     assert opt.gather_state([], index) == []
@@ -115,6 +117,9 @@ def test_group_options_and_torch_class(impl):
     import pickle
     other = pickle.loads(pickle.dumps(opt))
     assert other.param_groups[0]["state_bits"] == 8 and copy.deepcopy(opt).param_groups[0]["seed"] == 3
+    other.add_param_group({"params": [torch.nn.Parameter(torch.zeros(1))]})
+    assert other.param_groups[-1]["seed"] == 9 and other.last_grad_norm is None
+    assert len(opt.param_groups) == 2             # the refused group was not added
 
 
 def test_load_state_dict_keeps_types(impl):
@@ -187,7 +192,7 @@ def test_c_refusals_before_any_launch(impl):
              (dict(step_dev=at), {}, b"scalars"), (dict(), dict(scalars=at), b"scalars"), (dict(step_dev=at), dict(scalars=at + 4), b"aligned"),
              (dict(lr_dev=at), {}, b"lr on the device"), (dict(param=at + 2), {}, b"misaligned"), (dict(exp_avg_sq=at + 4), dict(bits=8), b"misaligned"),
              (dict(), dict(norm=at, max_norm=-1.0), b"max_norm"), (dict(), dict(norm=at, max_norm=float("nan")), b"max_norm"),
-             (dict(rows=1 << 41, row_len=1), {}, b"shape"), (dict(rows=1 << 32, row_len=1 << 20), {}, b"shape")]
+             (dict(rows=1 << 41, row_len=1), {}, b"shape"), (dict(rows=1 << 39, row_len=1), {}, b"workgroups"), (dict(rows=1 << 32, row_len=1 << 20), {}, b"shape")]
     for fields, args, message in cases:
         rc = step(tensor(**fields), **args)
         assert rc == -1 and message in lib.gs_last_error(), (fields, args, lib.gs_last_error())

@@ -316,6 +316,8 @@ def test_zero_and_non_finite_gradients(impl, dev, bits):
     opt.step()
     if bits == 8:                                 # the whole block of the NaN, the infinity's own element
         bad[64:128] = True
+        got = opt.unpacked([p])[0]
+        assert not got["exp_avg"][192:200].any()  # the infinity's neighbours start over while it is there
     assert torch.equal(p.detach().isnan(), bad)
     # a NaN norm reaches everything, as with torch.nn.utils.clip_grad_norm_
     q = torch.nn.Parameter(torch.ones(100, device=dev))
@@ -716,6 +718,19 @@ def test_bf16_parameter_keeps_small_updates_and_outside_writes(impl, dev):
         p.fill_(5.0)
     got = opt.unpacked([p])[0]["param"]
     assert float((got - 5.0).abs().max()) <= 5.0 * 2.0 ** -8
+    opt.state[p]["param_low"].copy_(torch.arange(-50, 50, dtype=torch.int16, device=dev) * 600)
+    for zero in (0.0, -0.0):                      # a remainder of the old value must not borrow through the sign
+        with torch.no_grad():
+            p.fill_(zero)
+        got = opt.unpacked([p])[0]["param"]
+        assert float(got.abs().max()) <= 2.0 ** -126            # half a step of bfloat16 at zero is a subnormal
+        q = torch.nn.Parameter(p.detach().clone())
+        twin = impl.FusedAdamW([q], lr=1e-5, weight_decay=0.5, state_bits=8)
+        twin.state[q] = {"step": torch.tensor(0.0), "moment_codes": torch.zeros(100, 2, dtype=torch.uint8, device=dev),
+                         "moment_scales": torch.zeros(2, 2, device=dev), "param_low": opt.state[p]["param_low"].clone()}
+        q.grad = torch.ones_like(q)
+        twin.step()
+        assert torch.equal(q.detach(), torch.full_like(q, -1e-5))
 
 
 # ---- together, as a training loop uses them -------------------------------------------------------------------------------
