@@ -104,6 +104,37 @@ def grad_norm(grads):
         return _norm([_matrix(g) for g in grads], dev, _stream(dev.index))
 
 
+class _Plan:
+    """One step's launches: packed descriptors by kernel form, and what has to live until they are made."""
+    __slots__ = ("dev", "params", "mats", "fresh", "counted", "keep", "buckets")
+
+    def __init__(self):
+        self.dev, self.params, self.mats, self.fresh, self.counted, self.keep, self.buckets = None, [], [], [], [], [], {}
+
+    def add(self, p, group, options, index, mat, state):
+        g, rows, row_len, stride = mat
+        lr_dev, lr, beta1, beta2, eps, weight_decay, seed = options
+        bits, on_gpu, step, step_dev, t = group["state_bits"], bool(group["capturable"]), state["step"], 0, 0
+        if on_gpu:
+            if not torch.is_tensor(step) or step.device != p.device or step.dtype is not _F32:
+                step = state["step"] = torch.as_tensor(step, dtype=_F32).to(p.device)
+            step_dev = step.data_ptr()
+        else:
+            t = int(step) + 1
+            self.counted.append((state, step, t))
+        if bits == 8:
+            a, b = state["moment_codes"], state["moment_scales"]
+        else:
+            a, b = state["exp_avg"], state["exp_avg_sq"]
+        bf16 = p.dtype is _BF16
+        key = (bf16, bits, group["stochastic_rounding"], on_gpu)
+        packed = self.buckets.get(key)
+        if packed is None:
+            packed = self.buckets[key] = []
+        packed.append(_STEP(p.data_ptr(), g.data_ptr(), state["param_low"].data_ptr() if bf16 else 0, a.data_ptr(), b.data_ptr(), step_dev, lr_dev,
+                            rows, stride, t, lr, beta1, beta2, eps, weight_decay, row_len, seed, index, 0))
+
+
 class FusedAdamW(torch.optim.AdamW):
     """AdamW on float32 or bfloat16 GPU parameters; see the module's docstring for what it adds to torch's class.
 
@@ -153,33 +184,48 @@ class FusedAdamW(torch.optim.AdamW):
                 raise ValueError("grad_norm is the norm that max_norm clips: give both")
         elif not float(max_norm) >= 0.0:
             raise ValueError(f"max_norm must not be negative, got {max_norm}")
-        work, dev = self._collect()
+        plan = self._plan()
         self.last_grad_norm = None
-        if not work:
+        dev = plan.dev
+        if dev is None:
             return loss
         if grad_norm is not None and (not torch.is_tensor(grad_norm) or grad_norm.device != dev or grad_norm.dtype is not _F32
                                       or grad_norm.numel() != 1):
             raise ValueError("grad_norm must be one float32 on the parameters' device")
         with _On(dev), _stage("adamw"):
-            if torch.cuda.is_current_stream_capturing():
-                self._check_capture(work)
+            if (plan.counted or plan.fresh) and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("FusedAdamW: a step that is captured needs capturable=True, or its counts would stay where they are at every replay"
+                                   if plan.counted or not all(group["capturable"] for _, group, _, _ in plan.fresh) else
+                                   "FusedAdamW: run one step before the capture: states made during it would be cleared by every replay")
+            for p, group, index, mat in plan.fresh:
+                state = self.state[p] = self._fresh_state(p, group["state_bits"], group["capturable"])
+                plan.add(p, group, self._options(group, dev, plan.keep), index, mat, state)
             stream = _stream(dev.index)
-            mats = [_matrix(w[3]) for w in work]
             if max_norm is not None and grad_norm is None:
-                grad_norm = _norm(mats, dev, stream)
-            self._launch(work, mats, grad_norm, max_norm, dev, stream)
+                grad_norm = _norm(plan.mats, dev, stream)
+            lib = _lib.load()
+            for (bf16, bits, stochastic, on_gpu), packed in plan.buckets.items():
+                scalars = torch.empty(4 * len(packed), dtype=_F32, device=dev) if on_gpu else None
+                _lib.check(lib.gs_adamw_step(len(packed), b"".join(packed), bf16, bits, stochastic, None if grad_norm is None else grad_norm.data_ptr(),
+                                             0.0 if max_norm is None else float(max_norm), None if scalars is None else scalars.data_ptr(),
+                                             stream), "gs_adamw_step")
+        for state, step, t in plan.counted:      # after the launches: a refused call leaves the counts as they were
+            if torch.is_tensor(step):
+                step.fill_(t)
+            else:
+                state["step"] = t
         self.last_grad_norm = grad_norm
-        torch.autograd.graph.increment_version([w[1] for w in work])
+        torch.autograd.graph.increment_version(plan.params)
         return loss
 
-    def _collect(self):
-        """Everything that the step updates, checked before anything changes: [(group, param, index, grad, state or None)]."""
-        work, dev, index, spans, states = [], None, -1, [], self.state
+    def _plan(self):
+        """Everything that the step updates, checked before anything changes."""
+        plan, dev, index, spans, states = _Plan(), None, -1, [], self.state
         for group in self.param_groups:
             if group["amsgrad"] or group["maximize"] or group["differentiable"]:
                 raise NotImplementedError("FusedAdamW: amsgrad / maximize / differentiable are not implemented")
             beta1, beta2 = group["betas"]
-            bits = group["state_bits"]
+            bits, options = group["state_bits"], None
             if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0 and group["eps"] >= 0.0 and bits in (8, 32)):
                 raise ValueError(f"FusedAdamW: betas {group['betas']}, eps {group['eps']}, state_bits {bits}: betas are in "
                                  "[0, 1), eps is not negative, state_bits is 8 or 32")
@@ -196,21 +242,42 @@ class FusedAdamW(torch.optim.AdamW):
                     dev = p.device
                 if g.dtype is not dtype or p.device != dev or g.device != dev:
                     raise RuntimeError("FusedAdamW: all parameters must live on one device, with gradients of their type there")
-                state = states.get(p) or None
-                if state is not None:
-                    self._check_state(p, state, bits)
                 n = p.numel()
                 if n:
                     start = p.data_ptr()
                     spans.append((start, start + n * (4 if dtype is _F32 else 2)))
-                work.append((group, p, index, g, state))
+                plan.params.append(p)
+                state = states.get(p) or None
+                if state is not None:
+                    self._check_state(p, state, bits)
+                mat = _matrix(g)
+                plan.mats.append(mat)
+                if state is None:
+                    plan.fresh.append((p, group, index, mat))
+                    continue
+                if options is None:
+                    options = self._options(group, dev, plan.keep)
+                plan.add(p, group, options, index, mat, state)
         spans.sort()
         end = 0
         for start, stop in spans:
             if start < end:
                 raise RuntimeError("FusedAdamW: two parameters share memory (or one is listed twice)")
             end = stop
-        return work, dev
+        plan.dev = dev
+        return plan
+
+    @staticmethod
+    def _options(group, dev, keep):
+        """What the descriptors of a group's tensors have in common: (lr_dev, lr, beta1, beta2, eps, weight_decay, seed)."""
+        lr, lr_dev = group["lr"], 0
+        if group["capturable"] and torch.is_tensor(lr) and lr.is_cuda:
+            lr = lr.detach().to(device=dev, dtype=_F32)
+            if lr.numel() != 1:
+                raise ValueError("FusedAdamW: lr must be one number")
+            keep.append(lr)
+            lr_dev, lr = lr.data_ptr(), 0.0
+        return (lr_dev, float(lr), *group["betas"], group["eps"], group["weight_decay"], group["seed"] & 0xFFFFFFFF)
 
     @staticmethod
     def _check_state(p, state, bits):
@@ -241,54 +308,6 @@ class FusedAdamW(torch.optim.AdamW):
         if p.dtype == torch.bfloat16:
             state["param_low"] = torch.zeros(p.shape, dtype=torch.int16, device=p.device)
         return state
-
-    @staticmethod
-    def _check_capture(work):
-        for group, p, _, _, state in work:
-            if not group["capturable"]:
-                raise RuntimeError("FusedAdamW: a step that is captured needs capturable=True (its counts would stay where they are at every replay)")
-            if state is None or not (torch.is_tensor(state["step"]) and state["step"].is_cuda):
-                raise RuntimeError("FusedAdamW: run one step before the capture (states made during a capture would be cleared by every replay)")
-
-    def _launch(self, work, mats, norm, max_norm, dev, stream):
-        lib = _lib.load()
-        buckets, keep, counted = {}, [], []
-        for (group, p, index, g, state), (gk, rows, row_len, stride) in zip(work, mats):
-            bits, on_gpu, bf16 = group["state_bits"], bool(group["capturable"]), p.dtype is _BF16
-            if state is None:
-                state = self.state[p] = self._fresh_state(p, bits, on_gpu)
-            lr, step, lr_dev, step_dev, t = group["lr"], state["step"], 0, 0, 0
-            if on_gpu:
-                if not torch.is_tensor(step) or step.device != dev or step.dtype is not _F32:
-                    step = state["step"] = torch.as_tensor(step, dtype=_F32).to(dev)
-                step_dev = step.data_ptr()
-                if torch.is_tensor(lr) and lr.is_cuda:
-                    lr = lr.detach().to(device=dev, dtype=_F32)
-                    if lr.numel() != 1:
-                        raise ValueError("FusedAdamW: lr must be one number")
-                    keep.append(lr)
-                    lr_dev, lr = lr.data_ptr(), 0.0
-            else:
-                t = int(step) + 1
-                counted.append((state, step, t))
-            a, b = (state["moment_codes"], state["moment_scales"]) if bits == 8 else (state["exp_avg"], state["exp_avg_sq"])
-            beta1, beta2 = group["betas"]
-            key = (bf16, bits, group["stochastic_rounding"], on_gpu)
-            if key not in buckets:
-                buckets[key] = []
-            buckets[key].append(_STEP(p.data_ptr(), gk.data_ptr(), state["param_low"].data_ptr() if bf16 else 0, a.data_ptr(), b.data_ptr(),
-                                      step_dev, lr_dev, rows, stride, t, float(lr), beta1, beta2, group["eps"], group["weight_decay"],
-                                      row_len, group["seed"] & 0xFFFFFFFF, index, 0))
-        for (bf16, bits, stochastic, on_gpu), packed in buckets.items():
-            scalars = torch.empty(4 * len(packed), dtype=_F32, device=dev) if on_gpu else None
-            _lib.check(lib.gs_adamw_step(len(packed), b"".join(packed), bf16, bits, stochastic, None if norm is None else norm.data_ptr(),
-                                         0.0 if max_norm is None else float(max_norm), None if scalars is None else scalars.data_ptr(),
-                                         stream), "gs_adamw_step")
-        for state, step, t in counted:           # after the launch: a refused call leaves the counts as they were
-            if torch.is_tensor(step):
-                step.fill_(t)
-            else:
-                state["step"] = t
 
     @torch.no_grad()
     def update_densify_stats(self, viewspace_grad=None, radii=None, xyz_gradient_accum=None, denom=None, max_radii2D=None):
@@ -404,39 +423,39 @@ class FusedAdamW(torch.optim.AdamW):
         out, packed, dev = [], [], None
         group_of = {q: group for group in self.param_groups for q in group["params"]} if states is None else None
         for p, s in pairs:
-            codes, got, numel = s.get("moment_codes"), {}, 0
-            entry = [0, 0, 0, 0, 0, 0, 0]
+            got, numel = {}, 0
+            codes = m = v = x = low = scales = 0          # addresses
             if p is not None and s:
                 if p not in group_of:
                     raise ValueError("not a parameter of this optimizer")
                 self._check_state(p, s, group_of[p]["state_bits"])
-            if codes is not None:
-                scales, here, numel = s["moment_scales"], codes.device, codes.numel() // 2
-                if p is None and (not (codes.is_cuda and codes.is_contiguous() and scales.is_contiguous()) or codes.dtype is not torch.uint8 or
-                                  scales.dtype is not _F32 or scales.device != here or codes.shape[-1:] != (2,) or
-                                  scales.shape != ((numel + BLOCK - 1) // BLOCK, 2)):
+            c = s.get("moment_codes")
+            if c is not None:
+                scale, here, numel = s["moment_scales"], c.device, c.numel() // 2
+                if p is None and (not (c.is_cuda and c.is_contiguous() and scale.is_contiguous()) or c.dtype is not torch.uint8 or
+                                  scale.dtype is not _F32 or scale.device != here or c.shape[-1:] != (2,) or
+                                  scale.shape != ((numel + BLOCK - 1) // BLOCK, 2)):
                     raise RuntimeError("unpacked: not a state of FusedAdamW on the GPU")
-                m = got["exp_avg"] = scales.new_empty(codes.shape[:-1])
-                v = got["exp_avg_sq"] = torch.empty_like(m)
-                entry[0], entry[1], entry[4], entry[5] = codes.data_ptr(), scales.data_ptr(), m.data_ptr(), v.data_ptr()
+                got["exp_avg"] = t = scale.new_empty(c.shape[:-1])
+                got["exp_avg_sq"] = w = torch.empty_like(t)
+                codes, scales, m, v = c.data_ptr(), scale.data_ptr(), t.data_ptr(), w.data_ptr()
             elif s:
                 got["exp_avg"], got["exp_avg_sq"] = s["exp_avg"], s["exp_avg_sq"]
+            bits16 = 0
             if p is not None:
-                got["param"] = p.detach()
-                if p.dtype is _BF16:
-                    if s:
-                        here, numel, low = p.device, p.numel(), s["param_low"]
-                        x = got["param"] = torch.empty(p.shape, dtype=_F32, device=here)
-                        entry[2], entry[3], entry[6] = p.data_ptr(), low.data_ptr(), x.data_ptr()
-                    else:
-                        got["param"] = p.detach().float()
+                if p.dtype is _F32 or not s:
+                    got["param"] = p.detach() if p.dtype is _F32 else p.detach().float()
+                else:
+                    here, numel = p.device, p.numel()
+                    got["param"] = t = torch.empty(p.shape, dtype=_F32, device=here)
+                    bits16, low, x = p.data_ptr(), s["param_low"].data_ptr(), t.data_ptr()
             out.append(got)
             if numel:
                 if dev is None:
                     dev = here
                 elif dev != here:
                     raise RuntimeError("unpacked: all tensors must live on one device")
-                packed.append(_UNPACK(*entry, numel))
+                packed.append(_UNPACK(codes, scales, bits16, low, m, v, x, numel))
         if packed:
             with _On(dev), _stage("adamw_unpack"):
                 _lib.check(_lib.load().gs_adamw_unpack(len(packed), b"".join(packed), _stream(dev.index)), "gs_adamw_unpack")
