@@ -104,8 +104,13 @@ def grad_norm(grads):
         return _norm([_matrix(g) for g in grads], dev, _stream(dev.index))
 
 
+def _counts_on(step, dev):
+    return torch.is_tensor(step) and step.dtype is _F32 and step.device == dev
+
+
 class _Plan:
-    """One step's launches: packed descriptors by kernel form, and what has to live until they are made."""
+    """One step's launches: packed descriptors by kernel form, what has to live until they are made, and the tensors (fresh) whose
+    state or count on the GPU has to be made first."""
     __slots__ = ("dev", "params", "mats", "fresh", "counted", "keep", "buckets")
 
     def __init__(self):
@@ -116,8 +121,6 @@ class _Plan:
         lr_dev, lr, beta1, beta2, eps, weight_decay, seed = options
         bits, on_gpu, step, step_dev, t = group["state_bits"], bool(group["capturable"]), state["step"], 0, 0
         if on_gpu:
-            if not torch.is_tensor(step) or step.device != p.device or step.dtype is not _F32:
-                step = state["step"] = torch.as_tensor(step, dtype=_F32).to(p.device)
             step_dev = step.data_ptr()
         else:
             t = int(step) + 1
@@ -196,9 +199,14 @@ class FusedAdamW(torch.optim.AdamW):
             if (plan.counted or plan.fresh) and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("FusedAdamW: a step that is captured needs capturable=True, or its counts would stay where they are at every replay"
                                    if plan.counted or not all(group["capturable"] for _, group, _, _ in plan.fresh) else
-                                   "FusedAdamW: run one step before the capture: states made during it would be cleared by every replay")
+                                   "FusedAdamW: run one step before the capture: states and counts made during it would be made again by every replay")
+            states = self.state
             for p, group, index, mat in plan.fresh:
-                state = self.state[p] = self._fresh_state(p, group["state_bits"], group["capturable"])
+                state = states.get(p) or None
+                if state is None:
+                    state = states[p] = self._fresh_state(p, group["state_bits"], group["capturable"])
+                elif group["capturable"]:
+                    state["step"] = torch.as_tensor(state["step"], dtype=_F32).to(dev)
                 plan.add(p, group, self._options(group, dev, plan.keep), index, mat, state)
             stream = _stream(dev.index)
             if max_norm is not None and grad_norm is None:
@@ -252,7 +260,7 @@ class FusedAdamW(torch.optim.AdamW):
                     self._check_state(p, state, bits)
                 mat = _matrix(g)
                 plan.mats.append(mat)
-                if state is None:
+                if state is None or group["capturable"] and not _counts_on(state["step"], dev):
                     plan.fresh.append((p, group, index, mat))
                     continue
                 if options is None:

@@ -588,6 +588,37 @@ def test_capture_refusals(impl, dev):
         assert torch.equal(p.detach(), before) and (capturable or float(opt.state[p]["step"]) == 1)
 
 
+def test_counts_move_to_the_gpu_outside_captures_only(impl, dev):
+    """capturable switched on for states that count on the host: refused during a capture, moved by the next eager step."""
+    p = torch.nn.Parameter(torch.ones(10, device=dev))
+    p.grad = torch.ones(10, device=dev)
+    opt = impl.FusedAdamW([p], lr=0.1)
+    opt.step()
+    opt.param_groups[0]["capturable"] = True
+    before = p.detach().clone()
+    with pytest.raises(RuntimeError, match="before the capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    torch.cuda.synchronize()
+    assert torch.equal(p.detach(), before) and not opt.state[p]["step"].is_cuda
+    opt.step()
+    assert opt.state[p]["step"].is_cuda and float(opt.state[p]["step"]) == 2
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    graph.replay()
+    torch.cuda.synchronize()
+    opt.param_groups[0]["capturable"] = False
+    opt.step()
+    assert float(opt.state[p]["step"]) == 4
+    q = torch.nn.Parameter(torch.ones(10, device=dev))
+    q.grad = torch.ones(10, device=dev)
+    ref = torch.optim.AdamW([q], lr=0.1)
+    for _ in range(4):
+        ref.step()
+    assert torch.equal(p, q)
+
+
 def test_steps_on_two_streams(impl, dev):
     """Two optimizers at once on streams of their own: no shared workspace."""
     gen = torch.Generator().manual_seed(1)
