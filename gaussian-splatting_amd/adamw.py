@@ -3,7 +3,7 @@
 ``FusedAdamW`` stands beside ``FusedAdam`` (optimizer.py) for training with decoupled weight decay: a
 ``torch.optim.AdamW`` whose ``step()`` is one HIP launch per 32 tensors (gs_adamw_step).  Beyond torch's class:
 
-    state_bits=8            two bytes of state per element instead of eight (a Gaussian model's moments: 472 -> 133 bytes per
+    state_bits=8            two bytes of state per element instead of eight (a Gaussian model's moments: 472 -> 125 bytes per
                             Gaussian of SH degree 3), rounded stochastically from a seed: the same seed gives the same bits
     step(max_norm=...)      clips by the global norm inside the step: no pass that rewrites the gradients
     bfloat16 parameters     the fp32 value is kept (16 more bits of state), so small updates are not lost
@@ -90,8 +90,8 @@ def grad_norm(grads):
     """sqrt of the sum of squares over all given tensors (None is skipped) as a 0-d float32 GPU tensor.
 
     float32 and bfloat16, any strides; accumulated in fp64 in a fixed order, so it neither overflows before its result does nor
-    depends on scheduling.  Nothing is synchronised.  For gradients sharded over ranks, all-reduce the square of the result
-    and pass its root to ``FusedAdamW.step(max_norm=..., grad_norm=...)``."""
+    depends on scheduling.  Nothing is synchronised.  For gradients sharded over ranks, pass the result through
+    ``parallel.reduce_grad_norm`` and on to ``FusedAdamW.step(max_norm=..., grad_norm=...)``."""
     grads = [grads] if torch.is_tensor(grads) else [g for g in grads if g is not None]
     if not grads:
         raise ValueError("grad_norm needs at least one tensor")
@@ -105,7 +105,7 @@ def grad_norm(grads):
 
 
 def _counts_on(step, dev):
-    return torch.is_tensor(step) and step.dtype is _F32 and step.device == dev
+    return torch.is_tensor(step) and step.dtype is _F32 and step.get_device() == dev.index
 
 
 class _Plan:
@@ -245,10 +245,11 @@ class FusedAdamW(torch.optim.AdamW):
                 dtype = p.dtype
                 if not p.is_cuda or dtype is not _F32 and dtype is not _BF16 or not p.is_contiguous():
                     raise RuntimeError("FusedAdamW needs contiguous float32 or bfloat16 parameters on the GPU (no CPU path)")
-                _check_grad(g, "FusedAdamW: a gradient")
+                if g.layout is not torch.strided:
+                    _check_grad(g, "FusedAdamW: a gradient")
                 if dev is None:
                     dev = p.device
-                if g.dtype is not dtype or p.device != dev or g.device != dev:
+                if g.dtype is not dtype or p.get_device() != dev.index or g.get_device() != dev.index:
                     raise RuntimeError("FusedAdamW: all parameters must live on one device, with gradients of their type there")
                 n = p.numel()
                 if n:
@@ -289,7 +290,7 @@ class FusedAdamW(torch.optim.AdamW):
 
     @staticmethod
     def _check_state(p, state, bits):
-        dev, shape = p.device, p.shape
+        dev, shape = p.get_device(), p.shape
         if bits == 8:
             a, b = state.get("moment_codes"), state.get("moment_scales")
             good = (a is not None and b is not None and a.dtype is torch.uint8 and a.shape == shape + (2,)
@@ -299,8 +300,8 @@ class FusedAdamW(torch.optim.AdamW):
             good = a is not None and b is not None and a.dtype is _F32 and a.shape == shape and b.shape == shape
         if p.dtype is _BF16:
             low = state.get("param_low")
-            good = good and low is not None and low.dtype is torch.int16 and low.shape == shape and low.is_contiguous() and low.device == dev
-        if not good or b.dtype is not _F32 or not (a.is_contiguous() and b.is_contiguous()) or a.device != dev or b.device != dev:
+            good = good and low is not None and low.dtype is torch.int16 and low.shape == shape and low.is_contiguous() and low.get_device() == dev
+        if not good or b.dtype is not _F32 or not (a.is_contiguous() and b.is_contiguous()) or a.get_device() != dev or b.get_device() != dev:
             raise RuntimeError(f"FusedAdamW: optimizer state does not match its parameter (shape {tuple(shape)}, {p.dtype}, state_bits {bits}); "
                                "replace_params() takes states along when rows are pruned or added")
 

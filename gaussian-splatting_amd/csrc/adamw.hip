@@ -340,6 +340,10 @@ __device__ __forceinline__ void adamw_chunk(const AwArgs& a, const AwTensor& T, 
     }
 }
 
+// Memory-bound in every form, one pass, everything read and written once (3 M Gaussians = 177 M elements, six tensors, the colour
+// gradients strided): fp32 with 32-bit moments 28 B an element, 0.95 ms = 5.2 TB/s; with 8-bit states 16.25 B, 0.53 ms = 5.4 TB/s at 101
+// VALU instructions an element, three quarters of the issue slots; a 2 GiB copy reaches 4.9 TB/s.  bf16 parameters (16 M elements):
+// 26 B in 64 us, 14.25 B in 46 us.
 template <bool BF16, bool Q8>
 __global__ __launch_bounds__(AW_THREADS) void adamw_kernel(const AwArgs a) {
     int ti = 0;
@@ -384,7 +388,8 @@ __global__ __launch_bounds__(64) void adamw_scalars_kernel(const AwScalarArgs a)
 // ---- sum of squares over many tensors -------------------------------------------------------------------------------
 // The order of the elements is free, so a lane takes a group of four elements of one row (contiguous tensors are one row): group j
 // starts at element 4 j, or at the row's fourth from last, and then leaves out what the group before it has.  No load
-// crosses a row, none depends on another, and all eight of a lane are under way before the first use.
+// crosses a row, none depends on another, and all eight of a lane are under way before the first use.  Bound by reading: 708 MB in
+// 0.12 ms = 5.7 TB/s (torch.sum reads at 4.0); doubles cost nothing beside that.
 constexpr int NRM_MAX_TENSORS = 48;
 constexpr int NRM_GROUPS = 2048;        // groups per workgroup and partial sum
 struct NrmTensor {
@@ -659,6 +664,9 @@ __device__ __forceinline__ void rows_short(const RowArgs& a, const RowTensor& T,
     }
 }
 
+// 3 M rows to 3 M, all six tensors: 32 bits 2.78 GB in 0.53 ms = 5.2 TB/s, memory-bound (one element a lane: 0.63 ms).  8 bits
+// 0.75 GB in 0.33 ms = 2.3 TB/s: bound by issue, 78 VALU instructions an element to unpack two codes with up to four scales a group,
+// find the new maxima and pack again.
 template <bool Q8>
 __global__ __launch_bounds__(AW_THREADS) void adamw_rows_kernel(const RowArgs a) {
     int ti = 0;
@@ -669,7 +677,8 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_rows_kernel(const RowArgs a)
     else rows_short<Q8>(a, T, base);
 }
 
-// ---- what packed states and split parameters stand for --------------------------------------------------------------
+// ---- what packed states and split parameters stand for ----------------------------------------------------------------
+// 2 B and a share of the scales read, 8 B written: 177 M elements in 0.30 ms = 6.0 TB/s.
 struct UnpackTensor { const uint16_t* codes; const float2* scales; const uint16_t* p; const int16_t* low; float* m; float* v; float* x; long long n; };
 struct UnpackArgs { UnpackTensor t[AW_MAX_TENSORS]; uint32_t block_begin[AW_MAX_TENSORS + 1]; int count; };
 

@@ -119,6 +119,17 @@ def reduce_densify_stats(xyz_gradient_accum: torch.Tensor, denom: torch.Tensor, 
     dist.all_reduce(max_radii2D, op=dist.ReduceOp.MAX, group=group)
 
 
+def reduce_grad_norm(norm: torch.Tensor, group: Optional[dist.ProcessGroup] = None) -> torch.Tensor:
+    """The gradient norm over all ranks from every rank's own, where each rank owns a shard of the Gaussians (SplatExchange):
+    sqrt of the sum of squares, in float64, so that the squares do not overflow.  What FusedAdamW.step(max_norm=...) takes as
+    ``grad_norm``; without it every rank would clip its shard by that shard's norm.  Replicated Gaussians need none."""
+    if not dist.is_initialized() or dist.get_world_size(group) == 1:
+        return norm
+    total = norm.detach().double().square().reshape(1)
+    _all_reduce_sum([total], group, async_op=False)
+    return total.sqrt().to(norm.dtype).reshape(norm.shape)
+
+
 def render_band(raster_settings, rank: int, world: int, t_eps=None, **inputs):
     """This rank's share of a tile-row sharded frame: renders only its band of 16-pixel tile rows.
 

@@ -42,7 +42,8 @@ extern "C" {
  * gradient rows, sh_jac rows) or a precondition changes: a binding compares gs_version() with the GS_ABI_VERSION it was
  * written against before its first call (gaussian-splatting_amd/_lib.py does) -- a mismatch means shifted arguments.
  * 100: round 1.  200: round 2 (sh_jac arguments, 64-byte gradient rows with six doubles, gs_identify_tile_ranges writes the
- * whole table and wants 16-byte aligned keys).  300: round 3.  303: this header (gs_preprocess_fwd_views and gs_preprocess_bwd_views added, gs_scan_tiles takes the sorted depth keys). */
+ * whole table and wants 16-byte aligned keys).  300: round 3.  303: this header (gs_preprocess_fwd_views and gs_preprocess_bwd_views added, gs_scan_tiles takes the sorted depth keys).
+ * gs_adamw_*, gs_grad_norm* were added to 303: nothing that was there changed, and a library without them fails to bind. */
 #define GS_ABI_VERSION 303
 int gs_version(void);            /* == GS_ABI_VERSION of the header the library was built from */
 const char* gs_last_error(void); /* message of this thread's last failing call */

@@ -277,3 +277,34 @@ def test_oracle_split_of_bf16():
     near = torch.from_numpy(x[:1000]).to(torch.bfloat16).float().numpy()
     got = torch.from_numpy(high[:1000].view(np.int16)).view(torch.bfloat16).float().numpy()
     assert np.all(np.abs(got - x[:1000]) <= np.abs(x[:1000]) * 2.0 ** -8) and (got != near).mean() < 0.01
+
+
+def _norm_worker(rank, world, port, tmp):
+    import sys
+    import torch.distributed as dist
+    sys.path.insert(0, ROOT)
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        par = importlib.import_module("gaussian-splatting_amd.parallel")
+        mine = torch.tensor([3.0, 4.0][rank])
+        got = par.reduce_grad_norm(mine)
+        assert got.shape == () and got.dtype == torch.float32 and float(got) == 5.0 and float(mine) == [3.0, 4.0][rank]
+        assert float(par.reduce_grad_norm(torch.tensor([3e30, 4e30][rank]))) == float(torch.tensor(5e30))       # the squares pass float32's range
+        assert torch.isnan(par.reduce_grad_norm(torch.tensor([1.0, float("nan")][rank])))
+        open(os.path.join(tmp, f"ok{rank}"), "w").write("ok")
+    finally:
+        dist.destroy_process_group()
+
+
+def test_norm_of_sharded_gradients_gloo(tmp_path):
+    import socket
+    import torch.multiprocessing as mp
+    s = socket.socket()
+    s.bind(("127.0.0.1", 0))
+    port = s.getsockname()[1]
+    s.close()
+    mp.spawn(_norm_worker, args=(2, port, str(tmp_path)), nprocs=2, join=True)
+    assert (tmp_path / "ok0").exists() and (tmp_path / "ok1").exists()
+    par = importlib.import_module("gaussian-splatting_amd.parallel")
+    assert float(par.reduce_grad_norm(torch.tensor(2.0))) == 2.0                                                 # no process group
