@@ -85,7 +85,7 @@ constexpr int GS_BWD_BATCH = GS_BWD_BATCH_DEF;           // pairs per backward b
 //   q2 = (red, green, blue, depth)
 // with A' = -0.5 log2e conic_a, B' = -log2e conic_b, C' = -0.5 log2e conic_d.  The box sits in one
 // 16-byte word (a visit is tested with q1 alone) and (red, green), (blue, depth) are aligned register
-// pairs for the forward's two pair-wise fmas (two v_fma_f32 each: the library is built without packed fp32 instructions).
+// pairs for the forward's two v_pk_fma_f32.
 __device__ __forceinline__ void to_lds_form(f4& p0, f4& p1, f4& p2) {
     const uint32_t rx = __float_as_uint(p1.w), ry = __float_as_uint(p2.w);
     p0.z *= -0.5f * GS_LOG2E;
