@@ -56,23 +56,23 @@ def _matrix(g):
     """(tensor to keep alive, rows, row length, row stride) of a gradient: rows that are contiguous in themselves are taken where they are."""
     if g.is_contiguous():
         return g, g.numel(), 1, 0
-    if g.shape[0] > 1:
+    shape, strides = g.shape, g.stride()
+    if shape[0] > 1:
         row_len = 1
-        for size, stride in zip(reversed(g.shape[1:]), reversed(g.stride()[1:])):
-            if size != 1 and stride != row_len:
+        for d in range(len(shape) - 1, 0, -1):
+            if strides[d] != row_len and shape[d] != 1:
                 break
-            row_len *= size
+            row_len *= shape[d]
         else:
-            if row_len <= g.stride(0) and 0 < row_len < 1 << 31:
-                return g, g.shape[0], row_len, g.stride(0)
+            if 0 < row_len <= strides[0] and row_len < 1 << 31:
+                return g, shape[0], row_len, strides[0]
     return g.detach().contiguous(), g.numel(), 1, 0
 
 
-def _check_grad(g, what):
+def _refuse_grad(g, what):
     if g.layout is not torch.strided or not g.is_cuda:
         raise RuntimeError(f"{what} must be a dense tensor on the GPU (no CPU path)")
-    if g.dtype is not _F32 and g.dtype is not _BF16:
-        raise RuntimeError(f"{what} must be float32 or bfloat16, not {g.dtype}")
+    raise RuntimeError(f"{what} must be float32 or bfloat16, not {g.dtype}")
 
 
 def _norm(mats, dev, stream):
@@ -97,8 +97,9 @@ def grad_norm(grads):
         raise ValueError("grad_norm needs at least one tensor")
     dev = grads[0].device
     for g in grads:
-        _check_grad(g, "grad_norm: a gradient")
-        if g.device != dev:
+        if g.layout is not torch.strided or not g.is_cuda or g.dtype is not _F32 and g.dtype is not _BF16:
+            _refuse_grad(g, "grad_norm: a gradient")
+        if g.get_device() != dev.index:
             raise RuntimeError("grad_norm: all gradients must live on one device")
     with _On(dev), _stage("grad_norm"):
         return _norm([_matrix(g) for g in grads], dev, _stream(dev.index))
@@ -246,7 +247,7 @@ class FusedAdamW(torch.optim.AdamW):
                 if not p.is_cuda or dtype is not _F32 and dtype is not _BF16 or not p.is_contiguous():
                     raise RuntimeError("FusedAdamW needs contiguous float32 or bfloat16 parameters on the GPU (no CPU path)")
                 if g.layout is not torch.strided:
-                    _check_grad(g, "FusedAdamW: a gradient")
+                    _refuse_grad(g, "FusedAdamW: a gradient")
                 if dev is None:
                     dev = p.device
                 if g.dtype is not dtype or p.get_device() != dev.index or g.get_device() != dev.index:
@@ -445,7 +446,7 @@ class FusedAdamW(torch.optim.AdamW):
                                   scale.dtype is not _F32 or scale.device != here or c.shape[-1:] != (2,) or
                                   scale.shape != ((numel + BLOCK - 1) // BLOCK, 2)):
                     raise RuntimeError("unpacked: not a state of FusedAdamW on the GPU")
-                got["exp_avg"] = t = scale.new_empty(c.shape[:-1])
+                got["exp_avg"] = t = torch.empty_like(p) if p is not None and p.dtype is _F32 else scale.new_empty(c.shape[:-1])
                 got["exp_avg_sq"] = w = torch.empty_like(t)
                 codes, scales, m, v = c.data_ptr(), scale.data_ptr(), t.data_ptr(), w.data_ptr()
             elif s:

@@ -871,3 +871,40 @@ def test_column_ranges_in_a_captured_step(impl, dev):
         runs.append(params)
     for p, q in zip(*runs):
         assert torch.equal(p, q)
+
+
+def test_unpacked_of_mixed_states(impl, dev):
+    """All kinds at once, empty tensors and missing states among them: every result is its own."""
+    gen = torch.Generator().manual_seed(11)
+    shapes = [(7, 3), (0, 3), (65,), (), (130, 2), (3, 0)]
+    groups, params = [], []
+    for bits in (8, 32):
+        for dtype in (torch.float32, torch.bfloat16):
+            ps = [torch.nn.Parameter(torch.randn(s, generator=gen).to(dev, dtype)) for s in shapes]
+            params += ps
+            groups.append({"params": ps, "state_bits": bits})
+    bare = torch.nn.Parameter(torch.ones(5, device=dev, dtype=torch.bfloat16))
+    opt = impl.FusedAdamW(groups + [{"params": [bare]}], lr=0.1)
+    for p in params:
+        p.grad = torch.randn(p.shape, generator=gen).to(dev, p.dtype)
+    opt.step()
+    got = opt.unpacked(params + [bare])
+    assert len(opt.unpacked()) == len(params) and set(got[-1]) == {"param"} and got[-1]["param"].dtype == torch.float32
+    for p, x in zip(params, got):
+        s = opt.state[p]
+        if "moment_codes" in s:
+            m, u = orc.unpack(_np(s["moment_codes"]).reshape(-1, 2), _np(s["moment_scales"]))
+            expect = m, u * u
+        else:
+            expect = _np(s["exp_avg"]).reshape(-1), _np(s["exp_avg_sq"]).reshape(-1)
+        for name, y in zip(("exp_avg", "exp_avg_sq"), expect):
+            assert x[name].shape == p.shape and x[name].dtype == torch.float32
+            assert np.array_equal(_np(x[name]).reshape(-1), y), name
+        value = orc.join(_bits16(p).reshape(-1), _np(s["param_low"]).reshape(-1)) if p.dtype == torch.bfloat16 else _np(p).reshape(-1)
+        assert x["param"].shape == p.shape and np.array_equal(_np(x["param"]).reshape(-1), value)
+    with pytest.raises(ValueError, match="not a parameter"):
+        stranger = torch.nn.Parameter(torch.ones(5, device=dev))
+        opt.state[stranger] = dict(opt.state[params[0]])
+        opt.unpacked([stranger])
+    with pytest.raises(RuntimeError, match="not a state"):
+        opt.unpacked(states=[{"moment_codes": torch.zeros(5, 2, device=dev), "moment_scales": torch.zeros(1, 2, device=dev)}])
