@@ -665,8 +665,9 @@ __device__ __forceinline__ void rows_short(const RowArgs& a, const RowTensor& T,
 }
 
 // 3 M rows to 3 M, all six tensors: 32 bits 2.78 GB in 0.53 ms = 5.2 TB/s, memory-bound (one element a lane: 0.63 ms).  8 bits
-// 0.75 GB in 0.33 ms = 2.3 TB/s: bound by issue, 78 VALU instructions an element to unpack two codes with up to four scales a group,
-// find the new maxima and pack again.
+// 0.75 GB in 0.33 ms = 2.3 TB/s: 78 VALU instructions an element to unpack two codes with up to four scales a group, find the new maxima
+// and pack again, behind a chain of three dependent loads (table, index, codes).  Neither alone is the bound: 8 % fewer
+// instructions gave 2 %, one or four groups a lane instead of two 360 and 376 us.
 template <bool Q8>
 __global__ __launch_bounds__(AW_THREADS) void adamw_rows_kernel(const RowArgs a) {
     int ti = 0;
